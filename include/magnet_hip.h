@@ -283,6 +283,93 @@ int mh_relu_bwd_to(const float* G, int64_t ld, int64_t im, const uint8_t* mask,
                    float* out, int64_t ldo, int64_t imo, int64_t n_rows, int32_t F, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits, and the weight gradient taken from them.  No counterpart in the reference, which keeps
+ * every activation of ChebConv.forward (src/layer/sparse_magnet.py:60-72) in 32 bits.
+ *
+ * A row-planar matrix of n_rows nodes and m columns is seen as R = 2 n_rows rows; 32 neighbouring columns of a row share a
+ * power-of-two scale.
+ *     codes  uint8 [R][mp], mp = m rounded up to 32: integer -127 .. 127 plus 128 (128 in the columns behind m)
+ *     scales uint8 [mp / 32][Rp], Rp = R rounded up to 8: exponent plus 128 (0 in the rows behind R); 255 marks a block that
+ *            held a value that was not finite and is restored as NaN
+ * A value is code * 2^exponent, off by at most half a step of its block: at most 1 / 127.5 of the block's largest magnitude.
+ * codes 4-byte, scales 8-byte aligned.
+ *   mh_ckpt_store    X -> codes, scales (all of both arrays is written)
+ *   mh_ckpt_restore  codes, scales -> X
+ *   mh_ckpt_gram     out[m][n] = A^T G, A the restored matrix [R][m], G row-planar float32 with n columns (stride 0 allowed):
+ *                    the weight gradient of a convolution whose propagated input is held in 8 bits.  Products and sums are
+ *                    float32; the same result every time.  A value of G that is not finite makes its column of out NaN.
+ *                    workspace: mh_ckpt_gram_workspace_bytes, contents irrelevant before and after.
+ */
+int mh_ckpt_store(const float* X, int64_t ld, int64_t im, int64_t n_rows, int32_t m, uint8_t* codes, uint8_t* scales,
+                  void* stream);
+int mh_ckpt_restore(const uint8_t* codes, const uint8_t* scales, int64_t n_rows, int32_t m, float* X, int64_t ld, int64_t im,
+                    void* stream);
+size_t mh_ckpt_gram_workspace_bytes(int64_t n_rows, int32_t m, int32_t n);
+int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t n_rows, int32_t m, const float* G, int64_t ldg, int64_t img,
+                 int32_t n, float* out /* [m][n] */, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Group norm of complex features over the graphs of a batch, with the complex ReLU behind it.  No counterpart in the
+ * reference, whose networks go from ChebConv to complex_relu_layer directly (src/layer/sparse_magnet.py:94-117); the gate
+ * is that layer's (:79-81).
+ *
+ * Graph b of the batch owns rows graph_ptr[b] .. graph_ptr[b+1] (DEVICE int32 [n_graphs + 1], from 0, not decreasing, at most
+ * n_rows; NULL: one graph of all rows).  Group g holds channels g F/groups .. (g+1) F/groups.  With m = mean z (complex) and
+ * v = mean |z - m|^2 over a graph's values of a group,
+ *     Y = gamma (X - m) / sqrt(v + eps) + beta on both parts  [relu: both parts times (Re Y >= 0)]
+ * gamma, beta: float[F] or NULL (1, 0).  Rows behind the last graph are written as zeros; a graph may be empty.
+ * stats: float[n_graphs * groups * MH_NORM_STATS], for the backward pass.  mask_out: uint8 [n_rows][F] or NULL, the gate.
+ *   mh_group_norm_bwd  dX, dgamma, dbeta (each may be NULL) from the gradient G of Y.  The input is X, or, where codes is not
+ *                      NULL, its checkpoint (mh_ckpt_store), with the gate from `mask` when relu (X is not read then).
+ * workspace: mh_group_norm_workspace_bytes, 8-byte aligned, contents irrelevant before and after.  Statistics and sums are
+ * held in 64 bits; the same result every time.
+ */
+#define MH_NORM_STATS 5
+size_t mh_group_norm_workspace_bytes(int64_t n_rows, int32_t n_graphs, int32_t F, int32_t groups);
+int mh_group_norm(const float* X, int64_t ld, int64_t im, int64_t n_rows, int32_t F, int32_t groups, const int32_t* graph_ptr,
+                  int32_t n_graphs, float eps, const float* gamma, const float* beta, int relu, float* Y, int64_t ldy, int64_t imy,
+                  uint8_t* mask_out, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+int mh_group_norm_bwd(const float* X, int64_t ld, int64_t im, const uint8_t* codes, const uint8_t* scales, const uint8_t* mask,
+                      int64_t n_rows, int32_t F, int32_t groups, const int32_t* graph_ptr, int32_t n_graphs, const float* stats,
+                      const float* gamma, const float* beta, int relu, const float* G, int64_t ldg, int64_t img, float* dX,
+                      int64_t lddx, int64_t imdx, float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Class scores -> log probabilities of given classes, entropy, top alternatives; mean NLL and accuracy.
+ * Replaces F.log_softmax + NLLLoss + max of the epoch loops (src/layer/sparse_magnet.py:128,163, src/sparse_Magnet.py:155-160,
+ * src/Edge_sparseMagnet.py:176-183), which the reference runs as separate passes over the scores.
+ *
+ * scores: dtype 0 float32, 1 bfloat16, 2 float16; element (b, c, i) at b sb + c sc + i sn, row (b, i) of n_batch * n_inner rows.
+ * labels: int64 [n_batch * n_inner] or NULL; a row whose label is `ignore` has log probability 0 and no gradient; any other
+ * label outside [0, n_classes) gives NaN.  Scores of -inf have probability 0; a row of nothing else, or one with +inf or NaN,
+ * gives NaN.  Computed in float32.
+ *   mh_class_logprobs  logprob[rows] (with labels), entropy[rows], the `top` (<= 16) best classes of a row at
+ *                      b tb + t tk + i tn of top_logprob / top_index: highest score first, ties to the lower class, NaN first.
+ *                      stat: float[2 * rows] for the backward pass, or NULL.
+ *   mh_class_logprobs_bwd  d_scores (type of the scores, strides db / dc / dn) from the gradients of logprob, entropy (strides
+ *                      0 or 1; NULL: none) and top_logprob (strides tb / tk / tn; NULL: none)
+ *   mh_class_nll       loss: mean of -log p over the rows that are not ignored; accuracy: share of them whose best class is the
+ *                      label; inv_count: 1 / their number (DEVICE scalars).  workspace: mh_class_nll_workspace_bytes().
+ *   mh_class_nll_bwd   d_scores from the gradient of the mean (DEVICE scalar)
+ */
+int mh_class_logprobs(const void* scores, int dtype, int64_t n_batch, int64_t n_inner, int32_t n_classes, int64_t sb, int64_t sc,
+                      int64_t sn, const int64_t* labels, int64_t ignore, float* logprob, float* entropy, float* stat, int32_t top,
+                      float* top_logprob, int64_t* top_index, int64_t tb, int64_t tk, int64_t tn, void* stream);
+int mh_class_logprobs_bwd(const void* scores, int dtype, int64_t n_batch, int64_t n_inner, int32_t n_classes, int64_t sb, int64_t sc,
+                          int64_t sn, const int64_t* labels, int64_t ignore, const float* stat, const float* entropy,
+                          const float* g_logprob, int64_t g_logprob_stride, const float* g_entropy, int64_t g_entropy_stride,
+                          int32_t top, const float* g_top, const int64_t* top_index, int64_t tb, int64_t tk, int64_t tn,
+                          void* d_scores, int64_t db, int64_t dc, int64_t dn, void* stream);
+size_t mh_class_nll_workspace_bytes(void);
+int mh_class_nll(const void* scores, int dtype, int64_t n_batch, int64_t n_inner, int32_t n_classes, int64_t sb, int64_t sc,
+                 int64_t sn, const int64_t* labels, int64_t ignore, float* stat, float* loss, float* accuracy,
+                 float* inv_count, void* workspace, size_t workspace_bytes, void* stream);
+int mh_class_nll_bwd(const void* scores, int dtype, int64_t n_batch, int64_t n_inner, int32_t n_classes, int64_t sb, int64_t sc,
+                     int64_t sn, const int64_t* labels, int64_t ignore, const float* stat, const float* inv_count, const float* g_loss,
+                     void* d_scores, int64_t db, int64_t dc, int64_t dn, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Halo exchange of a row-partitioned run, posted from native code over RCCL.  No counterpart in the
  * reference, which runs on one device (src/sparse_Magnet.py:23-24, src/Edge_sparseMagnet.py:148); it
  * serves the row partition that mh_lap_block_* and mh_halo_plan_* set up.

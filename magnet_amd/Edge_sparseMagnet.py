@@ -21,7 +21,7 @@ from .layer.sparse_magnet import ChebNet_Edge
 from .utils.edge_data import in_out_degree, generate_dataset_3class, link_prediction_evaluation, acc, split_cache_prefix
 from .utils.preprocess import to_edge_dataset_sparse
 from .utils.save_settings import write_log
-from .train import link_epoch, GraphedEpoch, SharedForwardEpochs, GraphedSharedEpochs
+from .train import link_epoch, GraphedEpoch, SharedForwardEpochs, GraphedSharedEpochs, save_report
 
 
 def parse_args(argv=None):
@@ -57,6 +57,17 @@ def parse_args(argv=None):
     parser.add_argument('--hip_graph', action='store_true',
                         help='(not in the reference) capture the epoch once and replay it as one HIP graph: the '
                              'small datasets spend their epoch in launch overhead')
+    parser.add_argument('--norm_groups', type=int, default=0,
+                        help='(not in the reference) a complex group norm of that many groups behind every convolution; '
+                             'must divide num_filter')
+    parser.add_argument('--checkpoint_bits', type=int, default=32, choices=(8, 32),
+                        help='(not in the reference) bits in which convolutions and norms keep what the backward pass '
+                             'needs of their input')
+    parser.add_argument('--fused_loss', action='store_true',
+                        help='(not in the reference) loss, accuracy and gradient from the class scores in one pass each way')
+    parser.add_argument('--report', type=int, default=0, metavar='TOP',
+                        help='(not in the reference) also write report{split}.npz: log probability of the label, entropy '
+                             'and the TOP best classes of every test pair under the best checkpoint')
     return parser.parse_args(argv)
 
 
@@ -104,7 +115,8 @@ def main(args):
         X_img = in_out_degree(edges, size, as_written=not args.true_degrees).to(device)
         X_real = X_img.clone()
         model = ChebNet_Edge(X_real.size(-1), L, None, K=args.K, label_dim=args.num_class_link, layer=args.layer,
-                             activation=args.activation, num_filter=args.num_filter, dropout=args.dropout).to(device)
+                             activation=args.activation, num_filter=args.num_filter, dropout=args.dropout, norm_groups=args.norm_groups,
+                             checkpoint_bits=args.checkpoint_bits).to(device)
         # the driver owns X_real / X_img and never writes them in place: keep the first layer's T_k(L) X across epochs
         model.Chebs[0].cache_input_propagation = True
         opt = optim.Adam(model.parameters(), lr=args.lr, weight_decay=args.l2, capturable=args.hip_graph)
@@ -112,11 +124,12 @@ def main(args):
         idx = {k: torch.from_numpy(np.asarray(datasets[i][k]['pairs'])).long().to(device) for k in ('train', 'validate', 'test')}
         best_test_err, early_stopping, log_str_full = 1000.0, 0, ''
         # one epoch of reference src/Edge_sparseMagnet.py:168-199: training step, then the validation forward
-        body = lambda: link_epoch(model, opt, X_real, X_img, idx['train'], y['train'], idx['validate'], y['validate'])
+        body = lambda: link_epoch(model, opt, X_real, X_img, idx['train'], y['train'], idx['validate'], y['validate'],
+                                  fused_loss=args.fused_loss)
         if not (args.hip_graph or args.separate_forwards):
             # same numbers, one pass through the convolutions per epoch: the validation forward is kept for the next
             # training step (same weights; pair gather and dropout act after the convolutions)
-            shared = SharedForwardEpochs(model, opt)
+            shared = SharedForwardEpochs(model, opt, fused_loss=args.fused_loss)
             body = lambda: shared.link_epoch(X_real, X_img, idx['train'], y['train'], idx['validate'], y['validate'])
         if args.hip_graph:
             # the capture's warm-up epochs are real optimizer steps: rewind parameters and Adam state in place
@@ -125,7 +138,7 @@ def main(args):
                 body = GraphedEpoch(body)
             else:                                     # the shared-forward epoch as two HIP graphs
                 body = GraphedSharedEpochs.for_links(model, opt, X_real, X_img, idx['train'], y['train'], idx['validate'],
-                                                     y['validate'])
+                                                     y['validate'], fused_loss=args.fused_loss)
             with torch.no_grad():
                 for p, p0 in zip(model.parameters(), start):
                     p.copy_(p0)
@@ -160,6 +173,8 @@ def main(args):
         row = []
         for name in ('/model', '/model_latest'):
             ov, ot = outputs(log_path + name + str(i) + '.t7')
+            if args.report and name == '/model':
+                save_report(log_path + '/report' + str(i), model, y['test'], args.report, X_real, X_img, idx['test'])
             if args.task != 2:
                 row += [acc(ov[:, :2].max(dim=1)[1], y['validate']), acc(ot[:, :2].max(dim=1)[1], y['test'])]
             else:

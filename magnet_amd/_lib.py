@@ -90,6 +90,32 @@ def _load():
     lib.mh_relu_bwd.argtypes = [vp, i64, i64, vp, i64, i32, vp]
     lib.mh_relu_bwd_to.restype = C.c_int
     lib.mh_relu_bwd_to.argtypes = [vp, i64, i64, vp, vp, i64, i64, i64, i32, vp]
+    lib.mh_ckpt_store.restype = C.c_int
+    lib.mh_ckpt_store.argtypes = [vp, i64, i64, i64, i32, vp, vp, vp]
+    lib.mh_ckpt_restore.restype = C.c_int
+    lib.mh_ckpt_restore.argtypes = [vp, vp, i64, i32, vp, i64, i64, vp]
+    lib.mh_ckpt_gram_workspace_bytes.restype = sz
+    lib.mh_ckpt_gram_workspace_bytes.argtypes = [i64, i32, i32]
+    lib.mh_ckpt_gram.restype = C.c_int
+    lib.mh_ckpt_gram.argtypes = [vp, vp, i64, i32, vp, i64, i64, i32, vp, vp, sz, vp]
+    lib.mh_group_norm_workspace_bytes.restype = sz
+    lib.mh_group_norm_workspace_bytes.argtypes = [i64, i32, i32, i32]
+    lib.mh_group_norm.restype = C.c_int
+    lib.mh_group_norm.argtypes = [vp, i64, i64, i64, i32, i32, vp, i32, f32, vp, vp, C.c_int, vp, i64, i64, vp, vp, vp, sz, vp]
+    lib.mh_group_norm_bwd.restype = C.c_int
+    lib.mh_group_norm_bwd.argtypes = [vp, i64, i64, vp, vp, vp, i64, i32, i32, vp, i32, vp, vp, vp, C.c_int, vp, i64, i64, vp, i64, i64,
+                                      vp, vp, vp, sz, vp]
+    lib.mh_class_logprobs.restype = C.c_int
+    lib.mh_class_logprobs.argtypes = [vp, C.c_int, i64, i64, i32, i64, i64, i64, vp, i64, vp, vp, vp, i32, vp, vp, i64, i64, i64, vp]
+    lib.mh_class_logprobs_bwd.restype = C.c_int
+    lib.mh_class_logprobs_bwd.argtypes = [vp, C.c_int, i64, i64, i32, i64, i64, i64, vp, i64, vp, vp, vp, i64, vp, i64, i32, vp, vp,
+                                          i64, i64, i64, vp, i64, i64, i64, vp]
+    lib.mh_class_nll_workspace_bytes.restype = sz
+    lib.mh_class_nll_workspace_bytes.argtypes = []
+    lib.mh_class_nll.restype = C.c_int
+    lib.mh_class_nll.argtypes = [vp, C.c_int, i64, i64, i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, sz, vp]
+    lib.mh_class_nll_bwd.restype = C.c_int
+    lib.mh_class_nll_bwd.argtypes = [vp, C.c_int, i64, i64, i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, i64, i64, i64, vp]
     lib.mh_cspmm_noalloc_init.restype = C.c_int
     lib.mh_cspmm_noalloc_init.argtypes = []
     lib.mh_cspmm_set_grid_cap.restype = C.c_int
@@ -120,7 +146,9 @@ lib = _load()
 # operators the extension registers (csrc/torch_ext.cpp)
 OPS = ['cspmm', 'cspmm_noalloc', 'plan_build', 'cheb_terms_', 'clenshaw', 'lap_build', 'lap_block_count',
        'lap_block_fill', 'pack', 'unpack',
-       'gather_rows', 'scatter_rows', 'bias_relu_', 'relu_bwd_', 'relu_bwd_out', 'halo_plan', 'powerlaw_edges', 'stream_read',
+       'gather_rows', 'scatter_rows', 'bias_relu_', 'relu_bwd_', 'relu_bwd_out',
+       'ckpt_store', 'ckpt_restore', 'ckpt_gram', 'group_norm', 'group_norm_bwd',
+       'class_logprobs', 'class_logprobs_bwd', 'class_nll', 'class_nll_bwd', 'halo_plan', 'powerlaw_edges', 'stream_read',
        'set_spmm_grid_cap', 'noalloc_init', 'exchange_new_id', 'exchange_create', 'exchange_begin', 'exchange_end',
        'exchange_all_gather', 'exchange_destroy', 'version']
 
@@ -161,6 +189,9 @@ EXPORTS = [
     'mh_cheb_terms', 'mh_clenshaw',
     'mh_halo_plan_workspace_bytes', 'mh_halo_plan_count', 'mh_halo_plan_fill',
     'mh_pack', 'mh_unpack', 'mh_gather_rows', 'mh_scatter_rows', 'mh_bias_relu', 'mh_relu_bwd', 'mh_relu_bwd_to',
+    'mh_ckpt_store', 'mh_ckpt_restore', 'mh_ckpt_gram_workspace_bytes', 'mh_ckpt_gram',
+    'mh_group_norm_workspace_bytes', 'mh_group_norm', 'mh_group_norm_bwd',
+    'mh_class_logprobs', 'mh_class_logprobs_bwd', 'mh_class_nll_workspace_bytes', 'mh_class_nll', 'mh_class_nll_bwd',
     'mh_exchange_id_bytes', 'mh_exchange_new_id', 'mh_exchange_create', 'mh_exchange_begin', 'mh_exchange_end',
     'mh_exchange_all_gather', 'mh_exchange_destroy',
     'mh_powerlaw_edges', 'mh_stream_read',

@@ -1,0 +1,406 @@
+// Activation checkpoints in 8 bits, and the weight gradient taken from them.
+//
+// Format.  A row-planar matrix [N][2][m] is seen as R = 2N rows of m columns; 32 neighbouring columns of a row share a
+// power-of-two scale 2^s.  With the block's largest magnitude f 2^p, f in [1/2, 1), s = p - 7, or p - 6 where rounding would
+// reach 128; -110 <= s <= 121.  code = rint(x / 2^s) (ties to even) lies in -127 .. 127 and is kept as code + 128.
+//     codes  uint8 [R][mp], mp = m rounded up to 32 (the columns behind m hold 128)
+//     scales uint8 [mp / 32][Rp], s + 128, Rp = R rounded up to 8 (the rows behind R hold 0); 255: a value of the block was not
+//            finite, and the whole block is restored as NaN
+// The error of a value is at most 2^s / 2: between 1 / 255 and 1 / 127.5 of its block's largest magnitude.  A power of
+// two costs up to one bit against a free scale and buys that code * 2^s is exact in bf16 (7 bits): the weight gradient runs on
+// the bf16 matrix cores without a further rounding of the activations.  The scales of 8 consecutive rows are 8 consecutive
+// bytes: one load for a thread that holds 8 rows of a block.
+#include <cstdint>
+
+#include <hip/hip_runtime.h>
+
+#include "ckpt.h"
+#include "common.h"
+
+namespace {
+
+using mhckpt::kBlockCols;
+constexpr int kBlock = 256;
+constexpr unsigned kMostBlocks = 1u << 16;
+
+// ---- store / restore -------------------------------------------------------------------------------------------------
+// A thread holds 4 columns of 8 consecutive rows (4 nodes): 8 independent 16-byte accesses, the 8 scales of its block as one
+// 8-byte word, written by the first of the 8 threads that share a block.  Bound by HBM.
+struct PlanarArgs {
+    float* x;
+    int64_t ld, im;
+    int64_t rows, rp;                       // rows = 2 N
+    int32_t m, mp;
+    uint8_t *codes, *scales;
+};
+
+template <bool VEC>
+__device__ inline float4 load4(const float* p, int32_t c, int32_t m) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (VEC) { if (c < m) v = *reinterpret_cast<const float4*>(p + c); }
+    else {
+        if (c < m) v.x = p[c];
+        if (c + 1 < m) v.y = p[c + 1];
+        if (c + 2 < m) v.z = p[c + 2];
+        if (c + 3 < m) v.w = p[c + 3];
+    }
+    return v;
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kBlock) ckpt_store_kernel(const PlanarArgs a) {
+    const int32_t quads = a.mp >> 2;
+    const int64_t total = (a.rp >> 3) * quads;                     // a multiple of 8: the 8 threads of a block stay together
+    for (int64_t t = int64_t(blockIdx.x) * kBlock + threadIdx.x; t < total; t += int64_t(gridDim.x) * kBlock) {
+        const int64_t oct = t / quads;
+        const int32_t c = int32_t(t - oct * quads) << 2;
+        const int64_t r0 = oct << 3;
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t r = r0 + k;
+            v[k] = r < a.rows ? load4<VEC>(a.x + (r >> 1) * a.ld + (k & 1) * a.im, c, a.m) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        uint64_t word = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            uint32_t top = mhckpt::magnitude(v[k]);
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) { const uint32_t other = __shfl_xor(top, o); top = other > top ? other : top; }
+            const uint32_t e = mhckpt::scale_byte(top);
+            if (r0 + k < a.rows) {
+                *reinterpret_cast<uint32_t*>(a.codes + (r0 + k) * a.mp + c) = mhckpt::encode(v[k], e);
+                word |= uint64_t(e) << (8 * k);
+            }
+        }
+        if ((c & (kBlockCols - 1)) == 0) *reinterpret_cast<uint64_t*>(a.scales + int64_t(c / kBlockCols) * a.rp + r0) = word;
+    }
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kBlock) ckpt_restore_kernel(const PlanarArgs a) {
+    const int32_t quads = (a.m + 3) >> 2;
+    const int64_t total = (a.rp >> 3) * quads;
+    for (int64_t t = int64_t(blockIdx.x) * kBlock + threadIdx.x; t < total; t += int64_t(gridDim.x) * kBlock) {
+        const int64_t oct = t / quads;
+        const int32_t c = int32_t(t - oct * quads) << 2;
+        const int64_t r0 = oct << 3;
+        const uint64_t word = *reinterpret_cast<const uint64_t*>(a.scales + int64_t(c / kBlockCols) * a.rp + r0);
+        uint32_t code[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) code[k] = r0 + k < a.rows ? *reinterpret_cast<const uint32_t*>(a.codes + (r0 + k) * a.mp + c) : 0u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (r0 + k >= a.rows) break;
+            const float4 v = mhckpt::decode(code[k], uint32_t(word >> (8 * k)) & 255u);
+            float* p = a.x + ((r0 + k) >> 1) * a.ld + (k & 1) * a.im;
+            if (VEC) *reinterpret_cast<float4*>(p + c) = v;
+            else {
+                p[c] = v.x;
+                if (c + 1 < a.m) p[c + 1] = v.y;
+                if (c + 2 < a.m) p[c + 2] = v.z;
+                if (c + 3 < a.m) p[c + 3] = v.w;
+            }
+        }
+    }
+}
+
+// ---- weight gradient -------------------------------------------------------------------------------------------------
+// out[i][j] = sum_r A[r][i] G[r][j]: A the decoded checkpoint [R][m], G float32 [R][n].
+//
+// A is exact in bf16; G is cut into three bf16 numbers g1 + g2 + g3 = g, each the next 8 bits of its significand (exact): three
+// bf16 matrix products with 32-bit sums give the float32 product at 3 / 16 of the cost of the float32 matrix instruction.
+//
+// The sum runs over millions of rows and the result is small, so the rows are cut into slabs; a workgroup takes one slab and
+// one BM x BN tile of the result and leaves a partial sum, a second kernel adds the slabs in order (64 bits; no atomics, the
+// same result every time).  Both operands are row-major and the sum runs down the rows, so a thread gathers 8 consecutive rows
+// of its columns (coalesced across the threads), converts them in registers and writes them to LDS as the 16 bytes that one
+// lane of the matrix instruction takes: layout [rows / 8][column][8], written and read as contiguous 16-byte accesses without
+// bank conflicts.  A thread decodes 4 neighbouring columns of A; column 4 u + q goes to place q BM / 4 + u (contiguous writes),
+// which permutes the rows of the tile and is undone when the slabs are added.  The next rows are loaded into registers before
+// the products of the current ones are issued; two workgroups share a CU and cover each other's conversion.
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+
+struct GramArgs {
+    const uint8_t *codes, *scales;
+    const float* g;
+    int64_t ldg, img, rows, rp, slab_rows;
+    int32_t m, mp, n, slabs, tiles_m, tiles_n;
+    float* partial;
+};
+
+// the high halves (bf16 by truncation) of two floats in one word
+__device__ inline uint32_t high_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
+__device__ inline float cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+
+template <int BM, int BN, int KT>
+__global__ void __launch_bounds__(kBlock, 2) ckpt_gram_kernel(const GramArgs a) {
+    constexpr int kg = KT / 8;
+    constexpr int na = (BM / 4 * kg + kBlock - 1) / kBlock, nb = (BN * kg + kBlock - 1) / kBlock;
+    constexpr int wn = BN >= 64 ? 2 : 1, wm = 4 / wn;               // waves across and down the tile
+    constexpr int mi = BM / 32 / wm, ni = BN / 32 / wn;             // 32 x 32 products of a wave
+    __shared__ __align__(16) uint16_t as[kg][BM][8];
+    __shared__ __align__(16) uint16_t bs[3][kg][BN][8];
+
+    // workgroups go to the XCDs in turn: the tiles of a slab are given to one XCD, whose L2 then serves the slab's rows to all
+    const int32_t tiles = a.tiles_m * a.tiles_n;
+    const int32_t slab = int32_t(blockIdx.x / (8 * tiles)) * 8 + int32_t(blockIdx.x & 7);
+    const int32_t tile = int32_t(blockIdx.x >> 3) % tiles;
+    if (slab >= a.slabs) return;
+    const int32_t i0 = (tile % a.tiles_m) * BM, j0 = (tile / a.tiles_m) * BN;
+    const int64_t r_end = (slab + 1) * a.slab_rows < a.rows ? (slab + 1) * a.slab_rows : a.rows;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wr = (wave / wn) * (BM / wm), wc = (wave % wn) * (BN / wn);
+
+    uint32_t code[na][8];
+    uint64_t word[na];
+    float gv[nb][8];
+    auto load = [&](int64_t r0) {
+#pragma unroll
+        for (int u = 0; u < na; ++u) {
+            const int t = u * kBlock + tid;
+            const int32_t c = i0 + (t % (BM / 4)) * 4;
+            const int64_t row = r0 + (t / (BM / 4)) * 8;
+            const bool in = t < BM / 4 * kg && c < a.mp;
+            word[u] = in && row < r_end ? *reinterpret_cast<const uint64_t*>(a.scales + int64_t(c / kBlockCols) * a.rp + row) : 0;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                code[u][q] = in && row + q < r_end ? *reinterpret_cast<const uint32_t*>(a.codes + (row + q) * a.mp + c) : 0x80808080u;
+        }
+#pragma unroll
+        for (int u = 0; u < nb; ++u) {
+            const int t = u * kBlock + tid;
+            const int32_t j = j0 + t % BN;
+            const int64_t row = r0 + (t / BN) * 8;
+            const bool in = t < BN * kg && j < a.n;
+            const float* p = a.g + (row >> 1) * a.ldg + j;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) gv[u][q] = in && row + q < r_end ? p[(q >> 1) * a.ldg + (q & 1) * a.img] : 0.0f;
+        }
+    };
+    auto stage = [&](int64_t r0) {
+#pragma unroll
+        for (int u = 0; u < na; ++u) {
+            const int t = u * kBlock + tid;
+            const int64_t left = r_end - (r0 + (t / (BM / 4)) * 8);
+            float4 v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = mhckpt::decode(code[u][q], q < left ? uint32_t(word[u] >> (8 * q)) & 255u : 1u);
+            if (t < BM / 4 * kg) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    u32x4 w;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float *x = &v[2 * q].x, *y = &v[2 * q + 1].x;
+                        w[q] = high_halves(x[c], y[c]);
+                    }
+                    *reinterpret_cast<u32x4*>(&as[t / (BM / 4)][c * (BM / 4) + t % (BM / 4)][0]) = w;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < nb; ++u) {
+            const int t = u * kBlock + tid;
+            u32x4 w[3];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float x1 = gv[u][2 * q], y1 = gv[u][2 * q + 1];
+                const float x2 = x1 - cut(x1), y2 = y1 - cut(y1);
+                const float x3 = x2 - cut(x2), y3 = y2 - cut(y2);
+                w[0][q] = high_halves(x1, y1);
+                w[1][q] = high_halves(x2, y2);
+                w[2][q] = high_halves(x3, y3);
+            }
+            if (t < BN * kg)
+#pragma unroll
+                for (int s = 0; s < 3; ++s) *reinterpret_cast<u32x4*>(&bs[s][t / BN][t % BN][0]) = w[s];
+        }
+    };
+
+    f32x16 acc[mi][ni];
+#pragma unroll
+    for (int i = 0; i < mi; ++i)
+#pragma unroll
+        for (int j = 0; j < ni; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
+
+    int64_t r0 = slab * a.slab_rows;
+    load(r0);
+    for (; r0 < r_end; r0 += KT) {
+        __syncthreads();                                           // the products of the rows before have read LDS
+        stage(r0);
+        __syncthreads();
+        if (r0 + KT < r_end) load(r0 + KT);
+#pragma unroll
+        for (int k = 0; k < kg; k += 2) {                           // 16 rows: lanes 0-31 take the first 8, lanes 32-63 the others
+            bf16x8 af[mi];
+#pragma unroll
+            for (int i = 0; i < mi; ++i) af[i] = *reinterpret_cast<const bf16x8*>(&as[k + (lane >> 5)][wr + i * 32 + (lane & 31)][0]);
+#pragma unroll
+            for (int j = 0; j < ni; ++j)
+#pragma unroll
+                for (int s = 2; s >= 0; --s) {                      // the smallest part first
+                    const bf16x8 bf = *reinterpret_cast<const bf16x8*>(&bs[s][k + (lane >> 5)][wc + j * 32 + (lane & 31)][0]);
+#pragma unroll
+                    for (int i = 0; i < mi; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[i], bf, acc[i][j], 0, 0, 0);
+                }
+        }
+    }
+    float* out = a.partial + (int64_t(slab) * tiles + tile) * (BM * BN);
+#pragma unroll
+    for (int i = 0; i < mi; ++i)
+#pragma unroll
+        for (int j = 0; j < ni; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                out[(wr + i * 32 + 8 * (k >> 2) + 4 * (lane >> 5) + (k & 3)) * BN + wc + j * 32 + (lane & 31)] = acc[i][j][k];
+}
+
+// the slabs' partial sums, in order; 64 results to a workgroup, its four waves take a quarter of the slabs each
+__global__ void __launch_bounds__(kBlock) ckpt_gram_join(const float* __restrict__ partial, int32_t slabs, int32_t tiles_m, int32_t tiles_n,
+                                                         int32_t bm, int32_t bn, int32_t m, int32_t n, float* __restrict__ out) {
+    __shared__ double part[kBlock / 64][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int32_t e = int32_t(blockIdx.x) * 64 + lane;
+    const bool in = e < m * n;
+    double sum = 0.0;
+    if (in) {
+        const int32_t i = e / n, j = e - i * n;
+        const int32_t tile = i / bm + (j / bn) * tiles_m, ii = i % bm;
+        const float* p = partial + int64_t(tile) * bm * bn + ((ii & 3) * (bm / 4) + (ii >> 2)) * bn + j % bn;
+        const int64_t step = int64_t(tiles_m) * tiles_n * bm * bn;
+        const int32_t s0 = int32_t(int64_t(slabs) * wave / 4), s1 = int32_t(int64_t(slabs) * (wave + 1) / 4);
+#pragma unroll 8
+        for (int32_t s = s0; s < s1; ++s) sum += double(p[s * step]);
+    }
+    part[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && in) out[e] = float(((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane]);
+}
+
+struct GramPlan {
+    int32_t bm, bn, kt, tiles_m, tiles_n, slabs;
+    int64_t slab_rows;
+};
+
+// Tile: the smallest that covers the result where it is small, 256 x 128 where it is not.  Slabs: two workgroups for each CU.
+GramPlan gram_plan(int64_t rows, int32_t m, int32_t n) {
+    GramPlan p;
+    const int32_t mp = (m + 31) & ~31;
+    p.bm = mp <= 128 || (mp > 256 && mp <= 384) ? 128 : 256;
+    p.bn = n <= 32 ? 32 : n <= 64 ? 64 : 128;
+    p.kt = p.bm == 256 ? 32 : 64;
+    p.tiles_m = (mp + p.bm - 1) / p.bm;
+    p.tiles_n = (n + p.bn - 1) / p.bn;
+    const int64_t want = (512 + p.tiles_m * p.tiles_n - 1) / (p.tiles_m * p.tiles_n);
+    int64_t each = (rows + want - 1) / want;
+    each = (each + p.kt - 1) / p.kt * p.kt;
+    p.slab_rows = each < p.kt ? p.kt : each;
+    p.slabs = int32_t((rows + p.slab_rows - 1) / p.slab_rows);
+    return p;
+}
+
+template <int BM, int BN, int KT>
+void launch_gram(const GramArgs& a, hipStream_t stream) {
+    const unsigned blocks = unsigned((a.slabs + 7) / 8 * 8) * unsigned(a.tiles_m * a.tiles_n);
+    ckpt_gram_kernel<BM, BN, KT><<<blocks, kBlock, 0, stream>>>(a);
+}
+
+unsigned grid_of(int64_t items) {
+    const int64_t b = (items + kBlock - 1) / kBlock;
+    return unsigned(b < 1 ? 1 : b > kMostBlocks ? kMostBlocks : b);
+}
+
+bool vec_ok(const float* x, int64_t ld, int64_t im, int32_t m) { return (m & 3) == 0 && (ld & 3) == 0 && (im & 3) == 0 && mh_aligned16(x); }
+
+int check_checkpoint(const void* codes, const void* scales, int64_t n_rows, int32_t m) {
+    MH_REQUIRE(n_rows >= 0 && m >= 1 && m <= (1 << 24), "n_rows=%lld m=%d", (long long)n_rows, m);
+    if (n_rows == 0) return MH_OK;
+    MH_REQUIRE(codes && scales, "null pointer");
+    MH_REQUIRE((reinterpret_cast<uintptr_t>(codes) & 3) == 0 && (reinterpret_cast<uintptr_t>(scales) & 7) == 0,
+               "codes must be 4-byte and scales 8-byte aligned");
+    return MH_OK;
+}
+
+PlanarArgs planar_args(float* x, int64_t ld, int64_t im, int64_t n_rows, int32_t m, uint8_t* codes, uint8_t* scales) {
+    PlanarArgs a{};
+    a.x = x; a.ld = ld; a.im = im; a.rows = 2 * n_rows; a.rp = (a.rows + 7) & ~int64_t(7); a.m = m; a.mp = (m + 31) & ~31;
+    a.codes = codes; a.scales = scales;
+    return a;
+}
+
+}  // namespace
+
+extern "C" int mh_ckpt_store(const float* X, int64_t ld, int64_t im, int64_t n_rows, int32_t m, uint8_t* codes, uint8_t* scales,
+                             void* stream_) {
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    if (int rc = check_checkpoint(codes, scales, n_rows, m)) return rc;
+    if (n_rows == 0) return MH_OK;
+    MH_REQUIRE(X, "null pointer");
+    MH_REQUIRE(ld >= 0 && im >= 0, "negative stride");
+    const PlanarArgs a = planar_args(const_cast<float*>(X), ld, im, n_rows, m, codes, scales);
+    const unsigned grid = grid_of((a.rp >> 3) * (a.mp >> 2));
+    if (vec_ok(X, ld, im, m)) ckpt_store_kernel<true><<<grid, kBlock, 0, stream>>>(a);
+    else ckpt_store_kernel<false><<<grid, kBlock, 0, stream>>>(a);
+    MH_LAUNCH_CHECK("ckpt_store");
+    return MH_OK;
+}
+
+extern "C" int mh_ckpt_restore(const uint8_t* codes, const uint8_t* scales, int64_t n_rows, int32_t m, float* X, int64_t ld, int64_t im,
+                               void* stream_) {
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    if (int rc = check_checkpoint(codes, scales, n_rows, m)) return rc;
+    if (n_rows == 0) return MH_OK;
+    MH_REQUIRE(X, "null pointer");
+    MH_REQUIRE(ld >= m && im >= m, "stride smaller than m");
+    const PlanarArgs a = planar_args(X, ld, im, n_rows, m, const_cast<uint8_t*>(codes), const_cast<uint8_t*>(scales));
+    const unsigned grid = grid_of((a.rp >> 3) * ((m + 3) >> 2));
+    if (vec_ok(X, ld, im, m)) ckpt_restore_kernel<true><<<grid, kBlock, 0, stream>>>(a);
+    else ckpt_restore_kernel<false><<<grid, kBlock, 0, stream>>>(a);
+    MH_LAUNCH_CHECK("ckpt_restore");
+    return MH_OK;
+}
+
+extern "C" size_t mh_ckpt_gram_workspace_bytes(int64_t n_rows, int32_t m, int32_t n) {
+    if (n_rows <= 0 || m < 1 || n < 1) return 0;
+    const GramPlan p = gram_plan(2 * n_rows, m, n);
+    return size_t(p.slabs) * p.tiles_m * p.tiles_n * p.bm * p.bn * sizeof(float);
+}
+
+extern "C" int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t n_rows, int32_t m, const float* G, int64_t ldg,
+                            int64_t img, int32_t n, float* out, void* workspace, size_t workspace_bytes, void* stream_) {
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    if (int rc = check_checkpoint(codes, scales, n_rows, m)) return rc;
+    MH_REQUIRE(n >= 1 && int64_t(m) * n <= (int64_t(1) << 30), "m=%d n=%d", m, n);
+    MH_REQUIRE(out, "null pointer");
+    MH_REQUIRE(ldg >= 0 && img >= 0, "negative stride");
+    GramArgs a{};
+    if (n_rows > 0) {
+        MH_REQUIRE(G && workspace, "null pointer");
+        const size_t need = mh_ckpt_gram_workspace_bytes(n_rows, m, n);
+        if (workspace_bytes < need) return mh::fail(MH_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    }
+    const GramPlan p = gram_plan(2 * n_rows, m, n);
+    a.codes = codes; a.scales = scales; a.g = G; a.ldg = ldg; a.img = img; a.rows = 2 * n_rows; a.rp = (a.rows + 7) & ~int64_t(7);
+    a.slab_rows = p.slab_rows; a.m = m; a.mp = (m + 31) & ~31; a.n = n; a.slabs = p.slabs; a.tiles_m = p.tiles_m; a.tiles_n = p.tiles_n;
+    a.partial = static_cast<float*>(workspace);
+    if (n_rows > 0) {
+        const int key = p.bm * 1000 + p.bn;
+        switch (key) {
+            case 128032: launch_gram<128, 32, 64>(a, stream); break;
+            case 128064: launch_gram<128, 64, 64>(a, stream); break;
+            case 128128: launch_gram<128, 128, 64>(a, stream); break;
+            case 256032: launch_gram<256, 32, 32>(a, stream); break;
+            case 256064: launch_gram<256, 64, 32>(a, stream); break;
+            default: launch_gram<256, 128, 32>(a, stream); break;
+        }
+        MH_LAUNCH_CHECK("ckpt_gram");
+    }
+    ckpt_gram_join<<<unsigned((int64_t(m) * n + 63) / 64), kBlock, 0, stream>>>(a.partial, a.slabs, a.tiles_m, a.tiles_n, p.bm, p.bn, m, n, out);
+    MH_LAUNCH_CHECK("ckpt_gram_join");
+    return MH_OK;
+}

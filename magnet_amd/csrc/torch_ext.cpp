@@ -11,6 +11,7 @@
 // `torch.ops.magnet.*` are the calls that replace them.
 #include <cstdint>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include <ATen/ATen.h>
@@ -381,6 +382,275 @@ void relu_bwd_out(const Tensor& G, const Tensor& mask, Tensor& out) {
              "relu_bwd_to");
 }
 
+// ---- 8-bit activation checkpoints --------------------------------------------------------------
+struct Held {
+    uint8_t *codes, *scales;
+    int64_t n, m;
+};
+
+// codes [2 n, m up to 32], scales [blocks, 2 n up to 8] of a checkpoint of [n, 2, m]
+Held held(const Tensor& codes, const Tensor& scales, int64_t n, int64_t m) {
+    need_cuda(codes, "codes"); need_cuda(scales, "scales");
+    TORCH_CHECK(n >= 0 && m >= 1 && m <= (1 << 24), "a checkpoint holds [n, 2, m] with m >= 1, got n=", n, " m=", m);
+    const int64_t mp = (m + 31) / 32 * 32, rp = (2 * n + 7) / 8 * 8;
+    TORCH_CHECK(codes.scalar_type() == at::kByte && codes.is_contiguous() && codes.dim() == 2 && codes.size(0) == 2 * n && codes.size(1) == mp,
+                "codes must be contiguous uint8 [", 2 * n, ", ", mp, "], got ", codes.scalar_type(), " ", codes.sizes());
+    TORCH_CHECK(scales.scalar_type() == at::kByte && scales.is_contiguous() && scales.dim() == 2 && scales.size(0) == mp / 32 && scales.size(1) == rp,
+                "scales must be contiguous uint8 [", mp / 32, ", ", rp, "], got ", scales.scalar_type(), " ", scales.sizes());
+    TORCH_CHECK(codes.device() == scales.device(), "codes and scales are on different devices");
+    return Held{codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), n, m};
+}
+
+void same_device(const Tensor& a, const Tensor& b, const char* name) {
+    TORCH_CHECK(a.device() == b.device(), name, " is on ", b.device().str(), ", the other operands on ", a.device().str());
+}
+
+void ckpt_store(const Tensor& X, Tensor& codes, Tensor& scales) {
+    const c10::DeviceGuard guard(X.device());
+    Planar x = planar(X, "X");
+    same_device(X, codes, "codes");
+    Held h = held(codes, scales, x.n, x.f);
+    check_rc(mh_ckpt_store(x.p, x.ld, x.im, x.n, int32_t(x.f), h.codes, h.scales, stream_of(X)), "ckpt_store");
+}
+
+void ckpt_restore(const Tensor& codes, const Tensor& scales, Tensor& out) {
+    const c10::DeviceGuard guard(out.device());
+    Planar x = planar(out, "out");
+    same_device(out, codes, "codes");
+    Held h = held(codes, scales, x.n, x.f);
+    check_rc(mh_ckpt_restore(h.codes, h.scales, x.n, int32_t(x.f), x.p, x.ld, x.im, stream_of(out)), "ckpt_restore");
+}
+
+// [m, n] float32
+Tensor ckpt_gram(const Tensor& codes, const Tensor& scales, int64_t m, const Tensor& G) {
+    const c10::DeviceGuard guard(G.device());
+    Planar g = planar(G, "G");
+    same_device(G, codes, "codes");
+    TORCH_CHECK(codes.dim() == 2 && codes.size(0) == 2 * g.n, "G has ", g.n, " rows, the checkpoint ", codes.dim() == 2 ? codes.size(0) / 2 : -1);
+    Held h = held(codes, scales, g.n, m);
+    TORCH_CHECK(g.f >= 1, "G has no columns");
+    const size_t bytes = mh_ckpt_gram_workspace_bytes(g.n, int32_t(m), int32_t(g.f));
+    Tensor out = at::empty({m, g.f}, G.options());
+    Tensor ws = at::empty({int64_t(bytes / sizeof(float))}, G.options());
+    check_rc(mh_ckpt_gram(h.codes, h.scales, g.n, int32_t(m), g.p, g.ld, g.im, int32_t(g.f), out.data_ptr<float>(), ws.data_ptr(), bytes,
+                          stream_of(G)), "ckpt_gram");
+    return out;
+}
+
+// ---- group norm --------------------------------------------------------------------------------
+struct Batch {
+    const int32_t* ptr = nullptr;
+    int32_t n = 1;
+};
+
+Batch batch_of(const OptTensor& graph_ptr, const Tensor& x, int64_t n) {
+    Batch b;
+    if (!graph_ptr.has_value() || !graph_ptr->defined()) { b.n = n ? 1 : 0; return b; }
+    b.ptr = i32(*graph_ptr, "graph_ptr");
+    same_device(x, *graph_ptr, "graph_ptr");
+    TORCH_CHECK(graph_ptr->dim() == 1 && graph_ptr->numel() >= 1 && graph_ptr->numel() <= (1 << 24), "graph_ptr must hold n_graphs + 1 row numbers");
+    b.n = int32_t(graph_ptr->numel() - 1);
+    return b;
+}
+
+const float* channels_of(const OptTensor& t, const char* name, const Tensor& x, int64_t f) {
+    if (!t.has_value() || !t->defined()) return nullptr;
+    need_cuda(*t, name);
+    same_device(x, *t, name);
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == f, name, " must be contiguous float32 with ", f,
+                " entries, got ", t->scalar_type(), " ", t->sizes());
+    return t->data_ptr<float>();
+}
+
+Tensor norm_workspace(const Tensor& x, int64_t n, int32_t graphs, int64_t f, int64_t groups) {
+    const size_t bytes = mh_group_norm_workspace_bytes(n, graphs, int32_t(f), int32_t(groups));
+    return at::empty({int64_t(bytes / sizeof(double) + 1)}, x.options().dtype(at::kDouble));
+}
+
+void check_groups(int64_t f, int64_t groups) {
+    TORCH_CHECK(f >= 1 && f <= (1 << 20) && groups >= 1 && f % groups == 0, f, " channels do not divide into ", groups, " groups");
+}
+
+// stats [n_graphs, groups, MH_NORM_STATS], for the backward pass
+Tensor group_norm(const Tensor& X, int64_t groups, const OptTensor& graph_ptr, double eps, const OptTensor& gamma, const OptTensor& beta,
+                  bool relu, Tensor& out, const OptTensor& mask) {
+    const c10::DeviceGuard guard(X.device());
+    Planar x = planar(X, "X"), y = planar(out, "out");
+    same_device(X, out, "out");
+    TORCH_CHECK(y.n == x.n && y.f == x.f, "out has shape ", out.sizes(), ", expected ", X.sizes());
+    check_groups(x.f, groups);
+    Batch b = batch_of(graph_ptr, X, x.n);
+    Tensor stats = at::empty({b.n, groups, MH_NORM_STATS}, X.options());
+    Tensor ws = norm_workspace(X, x.n, b.n, x.f, groups);
+    check_rc(mh_group_norm(x.p, x.ld, x.im, x.n, int32_t(x.f), int32_t(groups), b.ptr, b.n, float(eps), channels_of(gamma, "weight", X, x.f),
+                           channels_of(beta, "bias", X, x.f), relu ? 1 : 0, y.p, y.ld, y.im, mask_of(mask, x.n, x.f),
+                           stats.data_ptr<float>(), ws.data_ptr(), size_t(ws.numel()) * sizeof(double), stream_of(X)), "group_norm");
+    return stats;
+}
+
+void group_norm_bwd(const OptTensor& X, const OptTensor& codes, const OptTensor& scales, const OptTensor& mask, const Tensor& G,
+                    int64_t groups, const OptTensor& graph_ptr, const Tensor& stats, const OptTensor& gamma, const OptTensor& beta,
+                    bool relu, const OptTensor& dX, const OptTensor& dgamma, const OptTensor& dbeta) {
+    const c10::DeviceGuard guard(G.device());
+    Planar g = planar(G, "G");
+    check_groups(g.f, groups);
+    Planar x = planar_opt(X, "X", g.n, g.f), dx = planar_opt(dX, "dX", g.n, g.f);
+    uint8_t *c = nullptr, *s = nullptr;
+    if (codes.has_value() && codes->defined()) {
+        TORCH_CHECK(scales.has_value() && scales->defined(), "codes without scales");
+        same_device(G, *codes, "codes");
+        Held h = held(*codes, *scales, g.n, g.f);
+        c = h.codes; s = h.scales;
+    } else {
+        TORCH_CHECK(X.has_value() && X->defined(), "neither the input nor its checkpoint is given");
+        same_device(G, *X, "X");
+    }
+    Batch b = batch_of(graph_ptr, G, g.n);
+    need_cuda(stats, "stats");
+    TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == int64_t(b.n) * groups * MH_NORM_STATS,
+                "stats must be the tensor group_norm returned");
+    Tensor ws = norm_workspace(G, g.n, b.n, g.f, groups);
+    auto out = [&](const OptTensor& t, const char* name) { return const_cast<float*>(channels_of(t, name, G, g.f)); };
+    check_rc(mh_group_norm_bwd(x.p, x.ld, x.im, c, s, mask_of(mask, g.n, g.f), g.n, int32_t(g.f), int32_t(groups), b.ptr, b.n,
+                               stats.data_ptr<float>(), channels_of(gamma, "weight", G, g.f), channels_of(beta, "bias", G, g.f),
+                               relu ? 1 : 0, g.p, g.ld, g.im, dx.p, dx.ld, dx.im, out(dgamma, "dgamma"), out(dbeta, "dbeta"), ws.data_ptr(),
+                               size_t(ws.numel()) * sizeof(double), stream_of(G)), "group_norm_bwd");
+}
+
+// ---- class scores ------------------------------------------------------------------------------
+// scores [M, C], or [B, C, N] with the classes in the middle as the losses of torch have them
+struct Scores {
+    const void* p;
+    int dtype;
+    int64_t b, n, sb, sc, sn;
+    int32_t c;
+};
+
+Scores scores_of(const Tensor& t, const char* name) {
+    need_cuda(t, name);
+    TORCH_CHECK(t.dim() == 2 || t.dim() == 3, name, " must be [M, C] or [B, C, N], got ", t.sizes());
+    Scores s;
+    s.dtype = t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : t.scalar_type() == at::kHalf ? 2 : -1;
+    TORCH_CHECK(s.dtype >= 0, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+    TORCH_CHECK(t.size(1) >= 1 && t.size(1) <= (1 << 24), name, " has ", t.size(1), " classes");
+    s.p = t.data_ptr(); s.c = int32_t(t.size(1)); s.sc = t.stride(1);
+    if (t.dim() == 2) { s.b = 1; s.sb = 0; s.n = t.size(0); s.sn = t.stride(0); }
+    else { s.b = t.size(0); s.sb = t.stride(0); s.n = t.size(2); s.sn = t.stride(2); }
+    return s;
+}
+
+const int64_t* labels_of(const OptTensor& t, const Tensor& scores, int64_t rows) {
+    if (!t.has_value() || !t->defined()) return nullptr;
+    need_cuda(*t, "labels");
+    same_device(scores, *t, "labels");
+    TORCH_CHECK(t->scalar_type() == at::kLong && t->is_contiguous() && t->numel() == rows, "labels must be contiguous int64 with ", rows,
+                " entries, got ", t->scalar_type(), " ", t->sizes());
+    return t->data_ptr<int64_t>();
+}
+
+float* rows_of(const OptTensor& t, const char* name, const Tensor& scores, int64_t n) {
+    if (!t.has_value() || !t->defined()) return nullptr;
+    need_cuda(*t, name);
+    same_device(scores, *t, name);
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == n, name, " must be contiguous float32 with ", n, " entries");
+    return t->data_ptr<float>();
+}
+
+// gradient of one value per row: contiguous, or one value expanded over all rows
+std::pair<const float*, int64_t> row_grad(const OptTensor& t, const char* name, const Tensor& scores, int64_t n) {
+    if (!t.has_value() || !t->defined()) return {nullptr, 0};
+    need_cuda(*t, name);
+    same_device(scores, *t, name);
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->numel() == n, name, " must be float32 with ", n, " entries");
+    bool expanded = true;
+    for (int64_t d = 0; d < t->dim(); ++d) expanded = expanded && (t->size(d) <= 1 || t->stride(d) == 0);
+    TORCH_CHECK(expanded || t->is_contiguous(), name, " must be contiguous or one value expanded");
+    return {t->data_ptr<float>(), expanded ? 0 : 1};
+}
+
+struct Top {
+    int32_t k = 0;
+    int64_t tb = 0, tk = 0, tn = 0;
+};
+
+// [M, top] or [B, top, N], contiguous
+Top top_of(const OptTensor& t, const Tensor& scores, const Scores& s) {
+    Top r;
+    if (!t.has_value() || !t->defined()) return r;
+    need_cuda(*t, "top");
+    same_device(scores, *t, "top");
+    const bool flat = scores.dim() == 2;
+    TORCH_CHECK(t->dim() == scores.dim() && t->is_contiguous() && t->size(0) == scores.size(0) && (flat || t->size(2) == scores.size(2)),
+                "the top alternatives must be contiguous [M, top] or [B, top, N], got ", t->sizes());
+    TORCH_CHECK(t->size(1) <= 16 && t->size(1) <= s.c, "at most 16 alternatives and the number of classes (", s.c, "), asked for ", t->size(1));
+    r.k = int32_t(t->size(1));
+    if (flat) { r.tk = 1; r.tn = r.k; }
+    else { r.tb = r.k * s.n; r.tk = s.n; r.tn = 1; }
+    return r;
+}
+
+const int64_t* top_index_of(const OptTensor& index, const OptTensor& lp) {
+    if (!index.has_value() || !index->defined()) return nullptr;
+    TORCH_CHECK(lp.has_value() && lp->defined() && index->sizes() == lp->sizes() && index->scalar_type() == at::kLong && index->is_contiguous() &&
+                index->device() == lp->device(), "top_index must be contiguous int64 of top_logprob's shape");
+    return index->data_ptr<int64_t>();
+}
+
+void class_logprobs(const Tensor& scores, const OptTensor& labels, int64_t ignore, const OptTensor& logprob, Tensor& entropy,
+                    const OptTensor& stat, const OptTensor& top_lp, const OptTensor& top_index) {
+    const c10::DeviceGuard guard(scores.device());
+    Scores s = scores_of(scores, "scores");
+    const int64_t rows = s.b * s.n;
+    Top t = top_of(top_lp, scores, s);
+    int64_t* idx = const_cast<int64_t*>(top_index_of(top_index, top_lp));
+    TORCH_CHECK(t.k == 0 || (top_index.has_value() && top_index->defined()), "top_logprob without top_index");
+    if (top_lp.has_value() && top_lp->defined()) TORCH_CHECK(top_lp->scalar_type() == at::kFloat, "top_logprob must be float32");
+    check_rc(mh_class_logprobs(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, labels_of(labels, scores, rows), ignore,
+                               rows_of(logprob, "logprob", scores, rows), rows_of(entropy, "entropy", scores, rows),
+                               rows_of(stat, "stat", scores, 2 * rows), t.k, t.k ? top_lp->data_ptr<float>() : nullptr, idx, t.tb, t.tk, t.tn,
+                               stream_of(scores)), "class_logprobs");
+}
+
+void class_logprobs_bwd(const Tensor& scores, const OptTensor& labels, int64_t ignore, const Tensor& stat, const Tensor& entropy,
+                        const OptTensor& g_logprob, const OptTensor& g_entropy, const OptTensor& g_top, const OptTensor& top_index,
+                        Tensor& d_scores) {
+    const c10::DeviceGuard guard(scores.device());
+    Scores s = scores_of(scores, "scores"), d = scores_of(d_scores, "d_scores");
+    TORCH_CHECK(d_scores.sizes() == scores.sizes() && d.dtype == s.dtype && d_scores.device() == scores.device(), "d_scores must be like scores");
+    const int64_t rows = s.b * s.n;
+    Top t = top_of(g_top, scores, s);
+    if (t.k) TORCH_CHECK(g_top->scalar_type() == at::kFloat && top_index.has_value(), "g_top must be float32 and come with top_index");
+    auto gl = row_grad(g_logprob, "g_logprob", scores, rows), gh = row_grad(g_entropy, "g_entropy", scores, rows);
+    check_rc(mh_class_logprobs_bwd(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, labels_of(labels, scores, rows), ignore,
+                                   rows_of(stat, "stat", scores, 2 * rows), rows_of(entropy, "entropy", scores, rows), gl.first, gl.second,
+                                   gh.first, gh.second, t.k, t.k ? g_top->data_ptr<float>() : nullptr, t.k ? top_index_of(top_index, g_top) : nullptr,
+                                   t.tb, t.tk, t.tn, d_scores.data_ptr(), d.sb, d.sc, d.sn, stream_of(scores)), "class_logprobs_bwd");
+}
+
+void class_nll(const Tensor& scores, const Tensor& labels, int64_t ignore, const OptTensor& stat, Tensor& loss, Tensor& accuracy,
+               Tensor& inv_count) {
+    const c10::DeviceGuard guard(scores.device());
+    Scores s = scores_of(scores, "scores");
+    const int64_t rows = s.b * s.n;
+    const size_t bytes = mh_class_nll_workspace_bytes();
+    Tensor ws = at::empty({int64_t(bytes / sizeof(double))}, scores.options().dtype(at::kDouble));
+    check_rc(mh_class_nll(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, labels_of(labels, scores, rows), ignore,
+                          rows_of(stat, "stat", scores, 2 * rows), rows_of(loss, "loss", scores, 1),
+                          rows_of(accuracy, "accuracy", scores, 1), rows_of(inv_count, "inv_count", scores, 1), ws.data_ptr(), bytes, stream_of(scores)),
+             "class_nll");
+}
+
+void class_nll_bwd(const Tensor& scores, const Tensor& labels, int64_t ignore, const Tensor& stat, const Tensor& inv_count, const Tensor& g_loss,
+                   Tensor& d_scores) {
+    const c10::DeviceGuard guard(scores.device());
+    Scores s = scores_of(scores, "scores"), d = scores_of(d_scores, "d_scores");
+    TORCH_CHECK(d_scores.sizes() == scores.sizes() && d.dtype == s.dtype && d_scores.device() == scores.device(), "d_scores must be like scores");
+    const int64_t rows = s.b * s.n;
+    check_rc(mh_class_nll_bwd(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, labels_of(labels, scores, rows), ignore,
+                              rows_of(stat, "stat", scores, 2 * rows), rows_of(inv_count, "inv_count", scores, 1), rows_of(g_loss, "g_loss", scores, 1),
+                              d_scores.data_ptr(), d.sb, d.sc, d.sn, stream_of(scores)), "class_nll_bwd");
+}
+
 // launch width of the calling thread's following cspmm calls (0 = default)
 void set_spmm_grid_cap(int64_t workgroups) {
     TORCH_CHECK(workgroups >= 0 && workgroups <= INT32_MAX, "workgroups out of range");
@@ -525,6 +795,20 @@ TORCH_LIBRARY(magnet, m) {
     m.def("bias_relu_(Tensor(a!) Y, Tensor? bias, bool relu, Tensor(b!)? mask) -> ()");
     m.def("relu_bwd_(Tensor(a!) G, Tensor mask) -> ()");
     m.def("relu_bwd_out(Tensor G, Tensor mask, Tensor(a!) out) -> ()");
+    m.def("ckpt_store(Tensor X, Tensor(a!) codes, Tensor(b!) scales) -> ()");
+    m.def("ckpt_restore(Tensor codes, Tensor scales, Tensor(a!) out) -> ()");
+    m.def("ckpt_gram(Tensor codes, Tensor scales, int m, Tensor G) -> Tensor");
+    m.def("group_norm(Tensor X, int groups, Tensor? graph_ptr, float eps, Tensor? gamma, Tensor? beta, bool relu, Tensor(a!) out, "
+          "Tensor(b!)? mask) -> Tensor");
+    m.def("group_norm_bwd(Tensor? X, Tensor? codes, Tensor? scales, Tensor? mask, Tensor G, int groups, Tensor? graph_ptr, "
+          "Tensor stats, Tensor? gamma, Tensor? beta, bool relu, Tensor(a!)? dX, Tensor(b!)? dgamma, Tensor(c!)? dbeta) -> ()");
+    m.def("class_logprobs(Tensor scores, Tensor? labels, int ignore, Tensor(a!)? logprob, Tensor(b!) entropy, Tensor(c!)? stat, "
+          "Tensor(d!)? top_logprob, Tensor(e!)? top_index) -> ()");
+    m.def("class_logprobs_bwd(Tensor scores, Tensor? labels, int ignore, Tensor stat, Tensor entropy, Tensor? g_logprob, "
+          "Tensor? g_entropy, Tensor? g_top, Tensor? top_index, Tensor(a!) d_scores) -> ()");
+    m.def("class_nll(Tensor scores, Tensor labels, int ignore, Tensor(a!)? stat, Tensor(b!) loss, Tensor(c!) accuracy, "
+          "Tensor(d!) inv_count) -> ()");
+    m.def("class_nll_bwd(Tensor scores, Tensor labels, int ignore, Tensor stat, Tensor inv_count, Tensor g_loss, Tensor(a!) d_scores) -> ()");
     m.def("set_spmm_grid_cap(int workgroups) -> ()", &set_spmm_grid_cap);
     m.def("noalloc_init(int device_index) -> ()", &noalloc_init);
     m.def("halo_plan(Tensor col_idx, int n_cols, int c0, int c1, Tensor bounds) -> (Tensor, Tensor, Tensor)");
@@ -556,6 +840,15 @@ TORCH_LIBRARY_IMPL(magnet, CUDA, m) {
     m.impl("bias_relu_", &bias_relu_);
     m.impl("relu_bwd_", &relu_bwd_);
     m.impl("relu_bwd_out", &relu_bwd_out);
+    m.impl("ckpt_store", &ckpt_store);
+    m.impl("ckpt_restore", &ckpt_restore);
+    m.impl("ckpt_gram", &ckpt_gram);
+    m.impl("group_norm", &group_norm);
+    m.impl("group_norm_bwd", &group_norm_bwd);
+    m.impl("class_logprobs", &class_logprobs);
+    m.impl("class_logprobs_bwd", &class_logprobs_bwd);
+    m.impl("class_nll", &class_nll);
+    m.impl("class_nll_bwd", &class_nll_bwd);
     m.impl("halo_plan", &halo_plan);
     m.impl("powerlaw_edges", &powerlaw_edges);
     m.impl("stream_read", &stream_read);

@@ -41,6 +41,8 @@ Row partition
 import torch
 import torch.distributed as dist
 
+from ._lib import MagnetHipError
+
 
 # ---------------------------------------------------------------------------------------------
 # partition plan (plain tensor code: runs on CPU tensors for the gloo tests and on the GPU)
@@ -929,6 +931,23 @@ class _OrdersGemmFn(torch.autograd.Function):
         return dz, dw, db, None
 
 
+def _sharded_layers(net):
+    """(conv, relu follows) of a network that runs sharded."""
+    from .layer.norm import ComplexGroupNorm
+    from .layer.sparse_magnet import ChebConv, complex_relu_layer
+    mods, layers, i = list(net.Chebs), [], 0
+    if any(isinstance(m, ComplexGroupNorm) for m in mods):
+        raise MagnetHipError('sharded networks have no group norm: its statistics would span the ranks')
+    if any(getattr(m, 'checkpoint_bits', 32) != 32 for m in mods):
+        raise MagnetHipError('sharded networks keep their activations in 32 bits: checkpoint_bits must be 32')
+    while i < len(mods):
+        assert isinstance(mods[i], ChebConv)
+        relu = i + 1 < len(mods) and isinstance(mods[i + 1], complex_relu_layer)
+        layers.append((mods[i], relu))
+        i += 2 if relu else 1
+    return layers
+
+
 class ShardedChebNet:
     """Runs a ChebNet (magnet_amd.layer.sparse_magnet.ChebNet, same parameters / state_dict) on
     `world` GPUs.  Every rank holds the whole Laplacian; node features enter as row blocks.  Layers
@@ -954,19 +973,11 @@ class ShardedChebNet:
     _kept_pass = None
 
     def __init__(self, net, operator, n, rank, world, group=None):
-        from .layer.sparse_magnet import ChebConv, complex_relu_layer
         self.net, self.op, self.n, self.rank, self.world, self.group = net, operator, n, rank, world, group
         self._input_cache = None
         self.rb = [n * p // world for p in range(world)] + [n]
         self.r0, self.r1 = self.rb[rank], self.rb[rank + 1]
-        mods = list(net.Chebs)
-        self.layers = []
-        i = 0
-        while i < len(mods):
-            assert isinstance(mods[i], ChebConv)
-            relu = i + 1 < len(mods) and isinstance(mods[i + 1], complex_relu_layer)
-            self.layers.append((mods[i], relu))
-            i += 2 if relu else 1
+        self.layers = _sharded_layers(net)
 
     def _regroup(self, x, cb, to_cols):
         return _RegroupFn.apply(x, self.rb, cb, self.rank, self.world, self.group, to_cols)
@@ -1090,21 +1101,13 @@ class RowShardedChebNet(ShardedChebNet):
     rows per order — nothing of full height."""
 
     def __init__(self, net, part):
-        from .layer.sparse_magnet import ChebConv, complex_relu_layer
         self.net, self.part, self.n = net, part, part.n
         self.rank, self.world, self.group = part.rank, part.world, part.group
         self.rb = list(part.bounds)
         self.r0, self.r1 = part.r0, part.r1
         self.cache_input_propagation = False
         self._input_cache = None
-        mods = list(net.Chebs)
-        self.layers = []
-        i = 0
-        while i < len(mods):
-            assert isinstance(mods[i], ChebConv)
-            relu = i + 1 < len(mods) and isinstance(mods[i + 1], complex_relu_layer)
-            self.layers.append((mods[i], relu))
-            i += 2 if relu else 1
+        self.layers = _sharded_layers(net)
 
     def trunk(self, x_rows):
         from .layer.sparse_magnet import _ComplexReluFn

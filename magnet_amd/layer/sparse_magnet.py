@@ -9,6 +9,7 @@ reference src/layer/sparse_magnet.py:8-165:
     ChebNet(in_c, L_norm_real, L_norm_imag, num_filter, K, label_dim, activation, layer, dropout)
         .forward(real, imag)                      -> [1, label_dim, N]
     ChebNet_Edge(... same ...).forward(real, imag, index) -> [M, label_dim]
+                                                      (both nets: norm_groups, checkpoint_bits, graph_ptr on top)
     MagNetConv(in_c, out_c, K, q).forward(real, imag, edge_index, edge_weight=None)
 
 `L_norm_real` / `L_norm_imag` may be
@@ -36,6 +37,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .._lib import ops, MagnetHipError
+from ..checkpoint import Checkpoint8
 from ..laplacian import MagneticLaplacian, build_magnetic_laplacian, pack_complex, _packed_strides
 from ..utils.hermitian import ChebBasis
 
@@ -269,10 +271,12 @@ class _ChebConvFn(torch.autograd.Function):
 
     `in_block`: a block whose order 0 is xp and whose other orders this conv may fill (or that are
     filled already: `orders_ready`).  `next_terms`: allocate the output as order 0 of a block with that
-    many orders, for the conv that follows."""
+    many orders, for the conv that follows.  `bits` 8: what the weight gradient needs (the block of orders, or the input in
+    the GEMM-first form) is kept as a Checkpoint8 and the gradient taken from it; orders that the caller keeps anyway
+    (`orders_ready`) stay as they are."""
 
     @staticmethod
-    def forward(ctx, xp, weight, bias, lap, relu, in_block=None, orders_ready=False, next_terms=0):
+    def forward(ctx, xp, weight, bias, lap, relu, in_block=None, orders_ready=False, next_terms=0, bits=32):
         n, _, cin = xp.shape
         k1, _, cout = weight.shape
         w = weight.detach()
@@ -301,8 +305,11 @@ class _ChebConvFn(torch.autograd.Function):
             else:                                          # no activation pass: the bias rides on the GEMM
                 torch.addmm(b.reshape(1, cout), _block_rows(block), w.reshape(k1 * cin, cout), out=o2)
                 mask = None
-        ctx.x0 = None
-        if (block is not None and not orders_ready and RECOMPUTE_ORDERS_BYTES > 0
+        ctx.x0 = ctx.held = None
+        if bits == 8 and not orders_ready and ctx.needs_input_grad[1]:
+            ctx.held = Checkpoint8.store(xp if gemm_first else block)
+            block = None
+        elif (block is not None and not orders_ready and RECOMPUTE_ORDERS_BYTES > 0
                 and 8 * n * k1 * cin > RECOMPUTE_ORDERS_BYTES and ctx.needs_input_grad[1]):
             # keep the input only (a compact copy when it is order 0 of a handed-over block, which would
             # otherwise pin the whole block) and let the block go
@@ -312,7 +319,7 @@ class _ChebConvFn(torch.autograd.Function):
         ctx.mask = mask
         ctx.block = block
         ctx.shape = (n, cin)
-        ctx.save_for_backward(xp if gemm_first else None, weight)
+        ctx.save_for_backward(xp if gemm_first and ctx.held is None else None, weight)
         return out
 
     @staticmethod
@@ -337,7 +344,9 @@ class _ChebConvFn(torch.autograd.Function):
             if need_w or need_x:
                 _fill_orders(lap, ds)
             if need_w:                                     # X^T [T_0 G ... T_K G] -> [C_in, K+1, C_out]
-                dw = _gram(_rows2(xp), _block_rows(ds)).view(cin, k1, cout).permute(1, 0, 2).contiguous()
+                xg = _gram(_rows2(xp), _block_rows(ds)) if ctx.held is None else ctx.held.gram(ds)
+                dw = xg.view(cin, k1, cout).permute(1, 0, 2).contiguous()
+            ctx.held = None
             if need_x:
                 dx = torch.mm(_block_rows(ds), w.transpose(1, 2).reshape(k1 * cout, cin)).view(n, 2, cin)
         else:
@@ -345,11 +354,13 @@ class _ChebConvFn(torch.autograd.Function):
             if need_b:
                 db = _col_sums(g).view(1, cout)
             g2 = _rows2(g)
-            if need_w:
+            if need_w and ctx.held is not None:
+                dw = ctx.held.gram(g).view(k1, cin, cout)
+            elif need_w:
                 block = ctx.block if ctx.block is not None else _cheb_terms(lap, ctx.x0, k1)   # recomputed orders
                 dw = _gram(_block_rows(block), g2).view(k1, cin, cout)
                 block = None
-            ctx.block = ctx.x0 = None                      # the saved orders are not needed past this point
+            ctx.block = ctx.x0 = ctx.held = None                      # the saved orders are not needed past this point
             if need_x:
                 if 8 * n * k1 * cin <= FUSED_BACKWARD_BYTES:
                     ys = torch.mm(g2, w.permute(2, 0, 1).reshape(cout, k1 * cin)).view(n, 2, k1, cin)
@@ -357,7 +368,7 @@ class _ChebConvFn(torch.autograd.Function):
                 else:
                     # G W_k^T is formed when the recurrence reaches order k, not for all orders up front
                     dx, _ = _clenshaw(lap, lambda k: torch.mm(g2, w[k].t()).view(n, 2, cin), n_terms=k1)
-        return dx, dw, db, None, None, None, None, None
+        return dx, dw, db, None, None, None, None, None, None
 
 
 class _ChebTermsFn(torch.autograd.Function):
@@ -577,6 +588,13 @@ def _lap_from_pair(l_real, l_imag):
     return lap
 
 
+def _kept_bits(bits):
+    """Bits that a forward made now keeps its activations in."""
+    if bits not in (8, 32):
+        raise MagnetHipError('checkpoint_bits is 8 or 32, got %r' % (bits,))
+    return bits if torch.is_grad_enabled() else 32
+
+
 def _resolve_laplacian(L_norm_real, L_norm_imag):
     """-> ('cheb', MagneticLaplacian, n_terms or None) or ('list', [MagneticLaplacian...], n_terms)"""
     if isinstance(L_norm_real, ChebBasis):
@@ -641,6 +659,12 @@ class ChebConv(nn.Module):
     # RECOMPUTE_ORDERS_BYTES (when that budget is set) is never kept.
     cache_input_propagation = False
 
+    # What the weight gradient needs of the forward pass - the K+1 propagated orders of the input - in 8 bits instead of 32
+    # (magnet_amd.checkpoint.Checkpoint8: a quarter of the memory, values off by at most 1 / 127.5 of the largest of 32
+    # neighbours; forward results and the gradient of the input are not touched).  32 (default) or 8; convs over the
+    # reference's lists of matrices keep 32.  Takes the place of MH_RECOMPUTE_ORDERS_BYTES where both apply.
+    checkpoint_bits = 32
+
     def _spmm_first(self):
         """The ordering a conv in 'cheb' mode takes for a plain input: orders first when C_in <= C_out."""
         return self._mode == 'cheb' and self.weight.size(2) >= self.weight.size(1)
@@ -672,7 +696,7 @@ class ChebConv(nn.Module):
                 block, xp = None, pack_complex(real, imag)
             c = (real, imag, real._version, imag._version, xp, block, self._n_terms)
             self._input_cache = c
-        return _ChebConvFn.apply(c[4], w, self.bias, self._laps(), relu, c[5], c[5] is not None, next_terms)
+        return _ChebConvFn.apply(c[4], w, self.bias, self._laps(), relu, c[5], c[5] is not None, next_terms, 32)
 
     def forward_packed(self, xp, relu=False, next_terms=0, in_block=None):
         """Row-planar in, row-planar out; `relu` fuses the following complex ReLU.  `next_terms` > 1 makes
@@ -682,7 +706,8 @@ class ChebConv(nn.Module):
             raise MagnetHipError('%d Laplacian terms but weight has %d slices' % (self._n_terms, self.weight.size(0)))
         w = self.weight[:self._n_terms]
         if self._mode == 'cheb':
-            return _ChebConvFn.apply(xp, w, self.bias, self._laps(), relu, in_block, False, next_terms)
+            return _ChebConvFn.apply(xp, w, self.bias, self._laps(), relu, in_block, False, next_terms,
+                                     _kept_bits(self.checkpoint_bits))
         return _ListConvFn.apply(xp.contiguous(), w, self.bias, self._laps(), relu)
 
     def forward(self, data):
@@ -705,23 +730,28 @@ class complex_relu_layer(nn.Module):
         return self.complex_relu(real, img)
 
 
-def _run_trunk(chebs, real, imag):
-    """nn.Sequential of ChebConv / complex_relu_layer with each ReLU fused into the conv before it, and
-    each conv writing its output where the next conv wants its order 0."""
+def _run_trunk(chebs, real, imag, graph_ptr=None):
+    """nn.Sequential of ChebConv / ComplexGroupNorm / complex_relu_layer with each ReLU fused into the conv or norm before
+    it, and each of those writing its output where the next conv wants its order 0.  `graph_ptr`: the graphs that the norms
+    take their statistics over."""
+    from .norm import ComplexGroupNorm
     mods = list(chebs)
     p = None
     block = None                   # side-by-side block around p, made for the conv that consumes p
     i = 0
     while i < len(mods):
         m = mods[i]
-        if isinstance(m, ChebConv):
+        if isinstance(m, (ChebConv, ComplexGroupNorm)):
             fuse = i + 1 < len(mods) and isinstance(mods[i + 1], complex_relu_layer)
             step = 2 if fuse else 1
             nxt = mods[i + step] if i + step < len(mods) else None
             next_terms = nxt._n_terms if isinstance(nxt, ChebConv) and nxt._spmm_first() else 0
             if next_terms and 0 < RECOMPUTE_ORDERS_BYTES < 8 * real.size(0) * next_terms * nxt.weight.size(1):
                 next_terms = 0     # over the memory budget: blocks live one at a time, so none is allocated ahead
-            if p is None:
+            if isinstance(m, ComplexGroupNorm):
+                p = m.forward_packed(_as_packed(real, imag) if p is None else p, relu=fuse, graph_ptr=graph_ptr,
+                                     next_terms=next_terms)
+            elif p is None:
                 p = m.forward_first(real, imag, relu=fuse, next_terms=next_terms)
             else:
                 p = m.forward_packed(p, relu=fuse, next_terms=next_terms, in_block=block)
@@ -739,20 +769,33 @@ def _run_trunk(chebs, real, imag):
     return _as_packed(real, imag) if p is None else p
 
 
+def _network_layers(in_c, L_norm_real, L_norm_imag, num_filter, K, layer, activation, activate_first, norm_groups, checkpoint_bits):
+    """The convolutions of a network, each followed by its norm (norm_groups > 0) and its activation."""
+    from .norm import ComplexGroupNorm
+    chebs = []
+    for i in range(max(1, layer)):
+        conv = ChebConv(in_c=in_c if i == 0 else num_filter, out_c=num_filter, K=K, L_norm_real=L_norm_real,
+                        L_norm_imag=L_norm_imag)
+        conv.checkpoint_bits = checkpoint_bits
+        chebs.append(conv)
+        if norm_groups:
+            chebs.append(ComplexGroupNorm(norm_groups, num_filter, checkpoint_bits=checkpoint_bits))
+        if activation and (i > 0 or activate_first):
+            chebs.append(complex_relu_layer())
+    return chebs
+
+
 class ChebNet(nn.Module):
-    """Node-classification network (reference src/layer/sparse_magnet.py:94-130)."""
+    """Node-classification network (reference src/layer/sparse_magnet.py:94-130).  Not in the reference: `norm_groups` > 0 puts
+    a ComplexGroupNorm of that many groups behind every convolution, with statistics over each graph of `graph_ptr` (a batch
+    of graphs whose Laplacian is block-diagonal; None: one graph); `checkpoint_bits` 8 keeps what the backward pass needs
+    of convolutions and norms in 8 bits (ChebConv.checkpoint_bits)."""
 
     def __init__(self, in_c, L_norm_real, L_norm_imag, num_filter=2, K=2, label_dim=2, activation=False, layer=2,
-                 dropout=False):
+                 dropout=False, norm_groups=0, checkpoint_bits=32, graph_ptr=None):
         super(ChebNet, self).__init__()
-        chebs = [ChebConv(in_c=in_c, out_c=num_filter, K=K, L_norm_real=L_norm_real, L_norm_imag=L_norm_imag)]
-        if activation:
-            chebs.append(complex_relu_layer())
-        for i in range(1, layer):
-            chebs.append(ChebConv(in_c=num_filter, out_c=num_filter, K=K, L_norm_real=L_norm_real,
-                                  L_norm_imag=L_norm_imag))
-            if activation:
-                chebs.append(complex_relu_layer())
+        chebs = _network_layers(in_c, L_norm_real, L_norm_imag, num_filter, K, layer, activation, True, norm_groups, checkpoint_bits)
+        self.register_buffer('graph_ptr', graph_ptr, persistent=False)
         self.Chebs = torch.nn.Sequential(*chebs)
         last_dim = 2
         self.Conv = nn.Conv1d(num_filter * last_dim, label_dim, kernel_size=1)
@@ -762,16 +805,20 @@ class ChebNet(nn.Module):
         """The convolutions and activations: row-planar [N, 2, F] output of the last one.  Nothing in it depends
         on train / eval mode (dropout acts after it), so one trunk pass can serve an evaluation forward and the
         training forward that follows it under the same weights (magnet_amd.train.SharedForwardEpochs)."""
-        return _run_trunk(self.Chebs, real, imag)
+        return _run_trunk(self.Chebs, real, imag, self.graph_ptr)
 
-    def head(self, p):
-        """unwind -> dropout -> Conv1d(2F, label_dim, 1) -> log_softmax of a trunk output."""
+    def scores(self, p):
+        """unwind -> dropout -> Conv1d(2F, label_dim, 1) of a trunk output: class scores [1, label_dim, N], as
+        magnet_amd.layer.scores takes them."""
         x = p.reshape(p.size(0), -1)                   # == cat((real, imag), -1): same memory
         if self.dropout > 0:
             x = F.dropout(x, self.dropout, training=self.training)
         # Conv1d with kernel 1 over [1, 2F, N] is a linear map per node
-        x = _HeadFn.apply(x, self.Conv.weight.squeeze(-1), self.Conv.bias)          # [1, label_dim, N]
-        return F.log_softmax(x, dim=1)
+        return _HeadFn.apply(x, self.Conv.weight.squeeze(-1), self.Conv.bias)
+
+    def head(self, p):
+        """scores -> log_softmax of a trunk output."""
+        return F.log_softmax(self.scores(p), dim=1)
 
     def forward(self, real, imag):
         return self.head(self.trunk(real, imag))
@@ -779,19 +826,14 @@ class ChebNet(nn.Module):
 
 class ChebNet_Edge(nn.Module):
     """Link-prediction network (reference src/layer/sparse_magnet.py:133-165); `index` [M, 2] are
-    the node pairs to score."""
+    the node pairs to score.  `norm_groups`, `checkpoint_bits`, `graph_ptr` as in ChebNet."""
 
     def __init__(self, in_c, L_norm_real, L_norm_imag, num_filter=2, K=2, label_dim=2, activation=False, layer=2,
-                 dropout=False):
+                 dropout=False, norm_groups=0, checkpoint_bits=32, graph_ptr=None):
         super(ChebNet_Edge, self).__init__()
-        chebs = [ChebConv(in_c=in_c, out_c=num_filter, K=K, L_norm_real=L_norm_real, L_norm_imag=L_norm_imag)]
-        if activation and (layer != 1):
-            chebs.append(complex_relu_layer())
-        for i in range(1, layer):
-            chebs.append(ChebConv(in_c=num_filter, out_c=num_filter, K=K, L_norm_real=L_norm_real,
-                                  L_norm_imag=L_norm_imag))
-            if activation:
-                chebs.append(complex_relu_layer())
+        chebs = _network_layers(in_c, L_norm_real, L_norm_imag, num_filter, K, layer, activation, layer != 1, norm_groups,
+                                checkpoint_bits)
+        self.register_buffer('graph_ptr', graph_ptr, persistent=False)
         self.Chebs = torch.nn.Sequential(*chebs)
         last_dim = 2
         self.linear = nn.Linear(num_filter * last_dim * 2, label_dim)
@@ -799,15 +841,18 @@ class ChebNet_Edge(nn.Module):
 
     def trunk(self, real, imag):
         """The convolutions and activations (independent of train / eval mode and of the query pairs)."""
-        return _run_trunk(self.Chebs, real, imag)
+        return _run_trunk(self.Chebs, real, imag, self.graph_ptr)
 
-    def head(self, p, index):
-        """pair gather -> dropout -> Linear(4F, label_dim) -> log_softmax of a trunk output."""
+    def scores(self, p, index):
+        """pair gather -> dropout -> Linear(4F, label_dim) of a trunk output: class scores [M, label_dim]."""
         x = _PairGatherFn.apply(p, index)              # == cat(real[i], real[j], imag[i], imag[j])
         if self.dropout > 0:
             x = F.dropout(x, self.dropout, training=self.training)
-        x = self.linear(x)
-        return F.log_softmax(x, dim=1)
+        return self.linear(x)
+
+    def head(self, p, index):
+        """scores -> log_softmax of a trunk output."""
+        return F.log_softmax(self.scores(p, index), dim=1)
 
     def forward(self, real, imag, index):
         return self.head(self.trunk(real, imag), index)
@@ -817,6 +862,8 @@ class MagNetConv(nn.Module):
     """ChebConv that takes the graph at call time: forward(real, imag, edge_index, edge_weight=None).
     The magnetic Laplacian of (edge_index, edge_weight, q) is built on the GPU and cached until a
     different graph tensor is passed."""
+
+    checkpoint_bits = 32                               # as ChebConv's
 
     def __init__(self, in_c, out_c, K, q=0.25, bias=True):
         super(MagNetConv, self).__init__()
@@ -842,4 +889,5 @@ class MagNetConv(nn.Module):
 
     def forward(self, real, imag, edge_index, edge_weight=None):
         lap = self.laplacian(edge_index, edge_weight, real.size(0))
-        return _views(_ChebConvFn.apply(_as_packed(real, imag), self.weight, self.bias, lap, False, None, False, 0))
+        return _views(_ChebConvFn.apply(_as_packed(real, imag), self.weight, self.bias, lap, False, None, False, 0,
+                                        _kept_bits(self.checkpoint_bits)))

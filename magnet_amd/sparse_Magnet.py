@@ -22,7 +22,7 @@ import torch.optim as optim
 
 from . import data as D
 from .layer.sparse_magnet import ChebNet
-from .train import node_epoch, GraphedEpoch, NodeTargets, SharedForwardEpochs, GraphedSharedEpochs
+from .train import node_epoch, GraphedEpoch, NodeTargets, SharedForwardEpochs, GraphedSharedEpochs, save_report
 from .utils.preprocess import geometric_dataset_sparse
 from .utils.save_settings import write_log
 
@@ -60,6 +60,17 @@ def parse_args(argv=None):
     parser.add_argument('--hip_graph', action='store_true',
                         help='(not in the reference) capture the epoch once and replay it as one HIP graph: the '
                              'small datasets spend their epoch in launch overhead')
+    parser.add_argument('--norm_groups', type=int, default=0,
+                        help='(not in the reference) a complex group norm of that many groups behind every convolution; '
+                             'must divide num_filter')
+    parser.add_argument('--checkpoint_bits', type=int, default=32, choices=(8, 32),
+                        help='(not in the reference) bits in which convolutions and norms keep what the backward pass '
+                             'needs of their input')
+    parser.add_argument('--fused_loss', action='store_true',
+                        help='(not in the reference) loss, accuracy and gradient from the class scores in one pass each way')
+    parser.add_argument('--report', type=int, default=0, metavar='TOP',
+                        help='(not in the reference) also write report{split}.npz: log probability of the label, entropy '
+                             'and the TOP best classes of every node under the best checkpoint')
     return parser.parse_args(argv)
 
 
@@ -181,7 +192,8 @@ def main(args):
     for split in range(splits):
         log_str_full = ''
         model = ChebNet(X_real.size(-1), L, None, K=args.K, label_dim=cluster_dim, layer=args.layer,
-                        activation=args.activation, num_filter=args.num_filter, dropout=args.dropout).to(device)
+                        activation=args.activation, num_filter=args.num_filter, dropout=args.dropout, norm_groups=args.norm_groups,
+                        checkpoint_bits=args.checkpoint_bits).to(device)
         # the driver owns X_real / X_img and never writes them in place: keep the first layer's T_k(L) X across epochs
         model.Chebs[0].cache_input_propagation = True
         opt = optim.Adam(model.parameters(), lr=args.lr, weight_decay=args.l2, capturable=args.hip_graph)
@@ -191,11 +203,12 @@ def main(args):
         # the split's labels with the other nodes ignored: loss and accuracy of the reference's
         # criterion(preds[:, :, index], label[:, index]) without the per-epoch gather and index-put
         train_targets, val_targets = NodeTargets(label, train_index), NodeTargets(label, val_index)
-        body = lambda: node_epoch(model, opt, X_real, X_img, label, train_targets, val_targets, criterion)
+        body = lambda: node_epoch(model, opt, X_real, X_img, label, train_targets, val_targets, criterion,
+                                  fused_loss=args.fused_loss)
         if not (args.hip_graph or args.separate_forwards):
             # same numbers, one pass through the convolutions per epoch: the validation forward is kept for the next
             # training step (same weights; dropout acts after the convolutions)
-            shared = SharedForwardEpochs(model, opt)
+            shared = SharedForwardEpochs(model, opt, fused_loss=args.fused_loss)
             body = lambda: shared.node_epoch(X_real, X_img, label, train_targets, val_targets, criterion)
         if args.hip_graph:
             # the capture's warm-up epochs are real optimizer steps: rewind parameters and Adam state in place
@@ -203,7 +216,8 @@ def main(args):
             if args.separate_forwards:
                 body = GraphedEpoch(body)
             else:                                     # the shared-forward epoch as two HIP graphs
-                body = GraphedSharedEpochs.for_nodes(model, opt, X_real, X_img, label, train_targets, val_targets, criterion)
+                body = GraphedSharedEpochs.for_nodes(model, opt, X_real, X_img, label, train_targets, val_targets, criterion,
+                                                     fused_loss=args.fused_loss)
             with torch.no_grad():
                 for p, p0 in zip(model.parameters(), start):
                     p.copy_(p0)
@@ -243,6 +257,8 @@ def main(args):
 
         pred, acc_val, acc_test = evaluate(log_path + '/model' + str(split) + '.t7')
         np.save(log_path + '/pred' + str(split), pred.to('cpu'))
+        if args.report:
+            save_report(log_path + '/report' + str(split), model, label, args.report, X_real, X_img)
         pred, acc_val_latest, acc_test_latest = evaluate(log_path + '/model_latest' + str(split) + '.t7')
         np.save(log_path + '/pred_latest' + str(split), pred.to('cpu'))
         logstr = 'val_acc: ' + str(np.round(acc_val, 3)) + ' test_acc: ' + str(np.round(acc_test, 3)) + \
