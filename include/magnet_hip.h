@@ -289,8 +289,8 @@ int mh_relu_bwd_to(const float* G, int64_t ld, int64_t im, const uint8_t* mask,
  * A row-planar matrix of n_rows nodes and m columns is seen as R = 2 n_rows rows; 32 neighbouring columns of a row share a
  * power-of-two scale.
  *     codes  uint8 [R][mp], mp = m rounded up to 32: integer -127 .. 127 plus 128 (128 in the columns behind m)
- *     scales uint8 [mp / 32][Rp], Rp = R rounded up to 8: exponent plus 128 (0 in the rows behind R); 255 marks a block that
- *            held a value that was not finite and is restored as NaN
+ *     scales uint8 [mp / 32][Rp], Rp = R rounded up to 8: exponent plus 128 (0 in the rows behind R); 0 marks a block that
+ *            held a value that was not finite: its codes are 128 and it is restored as NaN
  * A value is code * 2^exponent, off by at most half a step of its block: at most 1 / 127.5 of the block's largest magnitude.
  * codes 4-byte, scales 8-byte aligned.
  *   mh_ckpt_store    X -> codes, scales (all of both arrays is written)

@@ -19,17 +19,15 @@ __device__ inline uint32_t magnitude(float4 v) {
 // scale byte s + 128 of a block whose largest magnitude has these bits: exponent field E means p = E - 126, so s = E - 133,
 // one more from 127.5 / 128 of the next power of two on
 __device__ inline uint32_t scale_byte(uint32_t top) {
-    if (top >= 0x7f800000u) return 255u;
+    if (top >= 0x7f800000u) return 0u;
     int s = int(top >> 23) - 133 + ((top & 0x7fffffu) >= 0x7f0000u ? 1 : 0);
     s = s < -110 ? -110 : s > 121 ? 121 : s;
     return uint32_t(s + 128);
 }
 
-// 2^s of a scale byte; NaN for 255, 0 for the bytes 0 and 1, which no block has
-__device__ inline float scale_of(uint32_t e) {
-    const uint32_t b = (e > 1u ? e - 1u : 0u) << 23;
-    return __uint_as_float(e == 255u ? 0x7fc00000u : b);
-}
+// 2^s of a scale byte: the exponent field is s + 127.  The byte 0 of a block that is not finite gives -inf, which its zero codes
+// turn into NaN; the byte 1, which no block has, gives 0.
+__device__ inline float scale_of(uint32_t e) { return __uint_as_float((e - 1u) << 23); }
 
 __device__ inline uint32_t encode1(float x, float inverse) {
     float q = rintf(x * inverse);
@@ -40,7 +38,7 @@ __device__ inline uint32_t encode1(float x, float inverse) {
 __device__ inline uint32_t encode(float4 v, uint32_t e) {
     // 1 / 2^s has the exponent field 127 - (e - 128) = 255 - e, between 6 and 237; a block that is not finite keeps no codes
     const float inverse = __uint_as_float((255u - e) << 23);
-    if (e == 255u) return 0x80808080u;
+    if (e == 0u) return 0x80808080u;
     return encode1(v.x, inverse) | (encode1(v.y, inverse) << 8) | (encode1(v.z, inverse) << 16) | (encode1(v.w, inverse) << 24);
 }
 

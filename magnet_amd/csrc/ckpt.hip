@@ -4,8 +4,8 @@
 // power-of-two scale 2^s.  With the block's largest magnitude f 2^p, f in [1/2, 1), s = p - 7, or p - 6 where rounding would
 // reach 128; -110 <= s <= 121.  code = rint(x / 2^s) (ties to even) lies in -127 .. 127 and is kept as code + 128.
 //     codes  uint8 [R][mp], mp = m rounded up to 32 (the columns behind m hold 128)
-//     scales uint8 [mp / 32][Rp], s + 128, Rp = R rounded up to 8 (the rows behind R hold 0); 255: a value of the block was not
-//            finite, and the whole block is restored as NaN
+//     scales uint8 [mp / 32][Rp], s + 128, Rp = R rounded up to 8 (the rows behind R hold 0); 0: a value of the block was not
+//            finite, and the whole block (of codes 128) is restored as NaN
 // The error of a value is at most 2^s / 2: between 1 / 255 and 1 / 127.5 of its block's largest magnitude.  A power of
 // two costs up to one bit against a free scale and buys that code * 2^s is exact in bf16 (7 bits): the weight gradient runs on
 // the bf16 matrix cores without a further rounding of the activations.  The scales of 8 consecutive rows are 8 consecutive
@@ -117,8 +117,13 @@ __global__ void __launch_bounds__(kBlock) ckpt_restore_kernel(const PlanarArgs a
 // of its columns (coalesced across the threads), converts them in registers and writes them to LDS as the 16 bytes that one
 // lane of the matrix instruction takes: layout [rows / 8][column][8], written and read as contiguous 16-byte accesses without
 // bank conflicts.  A thread decodes 4 neighbouring columns of A; column 4 u + q goes to place q BM / 4 + u (contiguous writes),
-// which permutes the rows of the tile and is undone when the slabs are added.  The next rows are loaded into registers before
-// the products of the current ones are issued; two workgroups share a CU and cover each other's conversion.
+// which permutes the rows of the tile and is undone when the slabs are added.
+//
+// A step takes 32 rows.  Its loads were issued three steps before, its conversion (2.5 instructions per value of A, 5.5 per
+// value of G) ran between the matrix instructions of the step before.  Conversion of G is repeated for every tile across A's
+// columns, hence the wide tiles: 2M x 384 with 128 columns of G takes 0.58 ms in one 384-wide tile, 1.27 ms in three of 128 with
+// one step in flight.  That is 1.0 PFLOP/s of bf16 products, what the library's largest bf16 product reaches on this card (1.1):
+// the matrix unit bounds it, at the clock it runs at under that load (1.9 GHz).  Narrow results (30 columns) run at 4.3 TB/s.
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
@@ -134,15 +139,22 @@ struct GramArgs {
 // the high halves (bf16 by truncation) of two floats in one word
 __device__ inline uint32_t high_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
 __device__ inline float cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+// address = uniform base + 32-bit offset of the thread: one load instruction, its base kept by the scalar unit
+template <class T>
+__device__ inline T at(const void* base, uint32_t offset) { return *reinterpret_cast<const T*>(static_cast<const char*>(base) + offset); }
 
-template <int BM, int BN, int KT>
-__global__ void __launch_bounds__(kBlock, 2) ckpt_gram_kernel(const GramArgs a) {
-    constexpr int kg = KT / 8;
-    constexpr int na = (BM / 4 * kg + kBlock - 1) / kBlock, nb = (BN * kg + kBlock - 1) / kBlock;
-    constexpr int wn = BN >= 64 ? 2 : 1, wm = 4 / wn;               // waves across and down the tile
-    constexpr int mi = BM / 32 / wm, ni = BN / 32 / wn;             // 32 x 32 products of a wave
-    __shared__ __align__(16) uint16_t as[kg][BM][8];
-    __shared__ __align__(16) uint16_t bs[3][kg][BN][8];
+constexpr int kRows = 32;                  // rows of a step
+constexpr int64_t kLeast = 128;          // rows of a slab: below, the sums to join cost more than the rows
+
+template <int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2) ckpt_gram_kernel(const GramArgs a) {
+    constexpr int threads = 64 * WM * WN, kg = kRows / 8;
+    constexpr int ta = BM / 4 * kg, tb = BN * kg;                   // conversion tasks of a step: 8 rows x 4 columns, 8 rows x 1
+    constexpr int na = (ta + threads - 1) / threads, nb = (tb + threads - 1) / threads;
+    constexpr int kFill = (na * 110 + nb * 60) / ((BM / 32 / WM) * (BN / 32 / WN) * 3 * kg / 2) + 1;
+    constexpr int mi = BM / 32 / WM, ni = BN / 32 / WN;             // 32 x 32 products of a wave
+    __shared__ __align__(16) uint16_t as[2][kg][BM][8];
+    __shared__ __align__(16) uint16_t bs[2][3][kg][BN][8];
 
     // workgroups go to the XCDs in turn: the tiles of a slab are given to one XCD, whose L2 then serves the slab's rows to all
     const int32_t tiles = a.tiles_m * a.tiles_n;
@@ -150,73 +162,102 @@ __global__ void __launch_bounds__(kBlock, 2) ckpt_gram_kernel(const GramArgs a) 
     const int32_t tile = int32_t(blockIdx.x >> 3) % tiles;
     if (slab >= a.slabs) return;
     const int32_t i0 = (tile % a.tiles_m) * BM, j0 = (tile / a.tiles_m) * BN;
-    const int64_t r_end = (slab + 1) * a.slab_rows < a.rows ? (slab + 1) * a.slab_rows : a.rows;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wr = (wave / wn) * (BM / wm), wc = (wave % wn) * (BN / wn);
+    const int64_t r_begin = slab * a.slab_rows;
+    const int64_t r_end = r_begin + a.slab_rows < a.rows ? r_begin + a.slab_rows : a.rows;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = (wave / WN) * (BM / WM), wc = (wave % WN) * (BN / WN);
 
-    uint32_t code[na][8];
-    uint64_t word[na];
-    float gv[nb][8];
-    auto load = [&](int64_t r0) {
+    uint32_t code[2][na][8];
+    uint64_t word[2][na];
+    float gv[2][nb][8];
+    // what lies behind the last column of A or G is read from the last one: its products end in places of the tile nobody reads
+    uint32_t offset_a[na], offset_b[nb];
+    const uint8_t* scale_at[na];
+    int k_a[na], k_b[nb];
+#pragma unroll
+    for (int u = 0; u < na; ++u) {
+        const int t = u * threads + tid;
+        int32_t c = i0 + (t % (BM / 4)) * 4;
+        c = c < a.mp ? c : a.mp - 4;
+        k_a[u] = t / (BM / 4) % kg;
+        offset_a[u] = uint32_t(k_a[u] * 8) * uint32_t(a.mp) + uint32_t(c);
+        scale_at[u] = a.scales + int64_t(c / kBlockCols) * a.rp + k_a[u] * 8;
+    }
+#pragma unroll
+    for (int u = 0; u < nb; ++u) {
+        const int t = u * threads + tid;
+        int32_t j = j0 + t % BN;
+        j = j < a.n ? j : a.n - 1;
+        k_b[u] = t / BN % kg;
+        offset_b[u] = (uint32_t(k_b[u] * 4) * uint32_t(a.ldg) + uint32_t(j)) * 4u;
+    }
+    // where there are fewer tasks than threads, the threads that are left do the first ones again and write the same: without
+    // branches a step is one block, in which conversions and products are scheduled into each other
+    auto load = [&](int set, int64_t r0) {
+        const uint8_t* codes = a.codes + r0 * a.mp;
+        const float* g = a.g + (r0 >> 1) * a.ldg;
 #pragma unroll
         for (int u = 0; u < na; ++u) {
-            const int t = u * kBlock + tid;
-            const int32_t c = i0 + (t % (BM / 4)) * 4;
-            const int64_t row = r0 + (t / (BM / 4)) * 8;
-            const bool in = t < BM / 4 * kg && c < a.mp;
-            word[u] = in && row < r_end ? *reinterpret_cast<const uint64_t*>(a.scales + int64_t(c / kBlockCols) * a.rp + row) : 0;
+            word[set][u] = *reinterpret_cast<const uint64_t*>(scale_at[u] + r0);
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-                code[u][q] = in && row + q < r_end ? *reinterpret_cast<const uint32_t*>(a.codes + (row + q) * a.mp + c) : 0x80808080u;
+            for (int q = 0; q < 8; ++q) code[set][u][q] = at<uint32_t>(codes + int64_t(q) * a.mp, offset_a[u]);
         }
 #pragma unroll
-        for (int u = 0; u < nb; ++u) {
-            const int t = u * kBlock + tid;
-            const int32_t j = j0 + t % BN;
-            const int64_t row = r0 + (t / BN) * 8;
-            const bool in = t < BN * kg && j < a.n;
-            const float* p = a.g + (row >> 1) * a.ldg + j;
+        for (int u = 0; u < nb; ++u)
 #pragma unroll
-            for (int q = 0; q < 8; ++q) gv[u][q] = in && row + q < r_end ? p[(q >> 1) * a.ldg + (q & 1) * a.img] : 0.0f;
-        }
+            for (int q = 0; q < 8; ++q) gv[set][u][q] = at<float>(g + (q >> 1) * a.ldg + (q & 1) * a.img, offset_b[u]);
     };
-    auto stage = [&](int64_t r0) {
+    // the rows behind the last whole step
+    auto load_rest = [&](int64_t r0) {
 #pragma unroll
         for (int u = 0; u < na; ++u) {
-            const int t = u * kBlock + tid;
-            const int64_t left = r_end - (r0 + (t / (BM / 4)) * 8);
-            float4 v[8];
-#pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = mhckpt::decode(code[u][q], q < left ? uint32_t(word[u] >> (8 * q)) & 255u : 1u);
-            if (t < BM / 4 * kg) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    u32x4 w;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float *x = &v[2 * q].x, *y = &v[2 * q + 1].x;
-                        w[q] = high_halves(x[c], y[c]);
-                    }
-                    *reinterpret_cast<u32x4*>(&as[t / (BM / 4)][c * (BM / 4) + t % (BM / 4)][0]) = w;
-                }
+            const int64_t left = r_end - (r0 + k_a[u] * 8);
+            word[0][u] = left > 0 ? *reinterpret_cast<const uint64_t*>(scale_at[u] + r0) : 0;
+            for (int q = 0; q < 8; ++q) {
+                code[0][u][q] = q < left ? at<uint32_t>(a.codes + (r0 + q) * a.mp, offset_a[u]) : 0x80808080u;
+                if (q >= left) word[0][u] = (word[0][u] & ~(uint64_t(255) << (8 * q))) | (uint64_t(1) << (8 * q));       // scale 0
             }
         }
 #pragma unroll
         for (int u = 0; u < nb; ++u) {
-            const int t = u * kBlock + tid;
+            const int64_t left = r_end - (r0 + k_b[u] * 8);
+            const float* g = a.g + (r0 >> 1) * a.ldg;
+            for (int q = 0; q < 8; ++q) gv[0][u][q] = q < left ? at<float>(g + (q >> 1) * a.ldg + (q & 1) * a.img, offset_b[u]) : 0.0f;
+        }
+    };
+    auto stage = [&](int set, int buf) {
+#pragma unroll
+        for (int u = 0; u < na; ++u) {
+            const int t = u * threads + tid;
+            float s[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) s[q] = mhckpt::scale_of(uint32_t(word[set][u] >> (8 * q)) & 255u);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) code[set][u][q] ^= 0x80808080u;                             // two's complement
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                u32x4 w;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    w[q] = high_halves(float(int8_t(code[set][u][2 * q] >> (8 * c))) * s[2 * q], float(int8_t(code[set][u][2 * q + 1] >> (8 * c))) * s[2 * q + 1]);
+                *reinterpret_cast<u32x4*>(&as[buf][t / (BM / 4) % kg][c * (BM / 4) + t % (BM / 4)][0]) = w;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < nb; ++u) {
+            const int t = u * threads + tid;
             u32x4 w[3];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float x1 = gv[u][2 * q], y1 = gv[u][2 * q + 1];
+                const float x1 = gv[set][u][2 * q], y1 = gv[set][u][2 * q + 1];
                 const float x2 = x1 - cut(x1), y2 = y1 - cut(y1);
                 const float x3 = x2 - cut(x2), y3 = y2 - cut(y2);
                 w[0][q] = high_halves(x1, y1);
                 w[1][q] = high_halves(x2, y2);
                 w[2][q] = high_halves(x3, y3);
             }
-            if (t < BN * kg)
 #pragma unroll
-                for (int s = 0; s < 3; ++s) *reinterpret_cast<u32x4*>(&bs[s][t / BN][t % BN][0]) = w[s];
+            for (int s = 0; s < 3; ++s) *reinterpret_cast<u32x4*>(&bs[buf][s][t / BN % kg][t % BN][0]) = w[s];
         }
     };
 
@@ -227,28 +268,58 @@ __global__ void __launch_bounds__(kBlock, 2) ckpt_gram_kernel(const GramArgs a) 
         for (int j = 0; j < ni; ++j)
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
+    auto product = [&](int buf, int k) {                            // 16 rows: lanes 0-31 take the first 8, lanes 32-63 the others
+        bf16x8 af[mi];
+#pragma unroll
+        for (int i = 0; i < mi; ++i) af[i] = *reinterpret_cast<const bf16x8*>(&as[buf][k + (lane >> 5)][wr + i * 32 + (lane & 31)][0]);
+#pragma unroll
+        for (int j = 0; j < ni; ++j)
+#pragma unroll
+            for (int s = 2; s >= 0; --s) {                          // the smallest part first
+                const bf16x8 bf = *reinterpret_cast<const bf16x8*>(&bs[buf][s][k + (lane >> 5)][wc + j * 32 + (lane & 31)][0]);
+#pragma unroll
+                for (int i = 0; i < mi; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[i], bf, acc[i][j], 0, 0, 0);
+            }
+    };
 
-    int64_t r0 = slab * a.slab_rows;
-    load(r0);
-    for (; r0 < r_end; r0 += KT) {
-        __syncthreads();                                           // the products of the rows before have read LDS
-        stage(r0);
+    // LDS holds two steps: while the products of one are made, the next is converted into the other half, and the two after
+    // that are on their way into registers.  Past the last whole step the loads repeat it and what they bring is not used.
+    const int64_t whole = (r_end - r_begin) / kRows;
+    if (whole > 0) {
+        const int64_t last = r_begin + (whole - 1) * kRows;
+        auto row = [&](int64_t k) { const int64_t r = r_begin + k * kRows; return r < last ? r : last; };
+        auto step = [&](int buf, int64_t k) {
+            product(buf, 0);
+            stage(buf ^ 1, buf ^ 1);
+            load(buf ^ 1, row(k + 3));
+            product(buf, 2);
+            // a matrix instruction, then what the vector unit can do while it runs
+#pragma unroll
+            for (int i = 0; i < mi * ni * 3 * kg / 2; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, kFill, 0);
+            }
+            __syncthreads();
+        };
+        load(0, row(0));
+        load(1, row(1));
+        stage(0, 0);
+        load(0, row(2));
         __syncthreads();
-        if (r0 + KT < r_end) load(r0 + KT);
-#pragma unroll
-        for (int k = 0; k < kg; k += 2) {                           // 16 rows: lanes 0-31 take the first 8, lanes 32-63 the others
-            bf16x8 af[mi];
-#pragma unroll
-            for (int i = 0; i < mi; ++i) af[i] = *reinterpret_cast<const bf16x8*>(&as[k + (lane >> 5)][wr + i * 32 + (lane & 31)][0]);
-#pragma unroll
-            for (int j = 0; j < ni; ++j)
-#pragma unroll
-                for (int s = 2; s >= 0; --s) {                      // the smallest part first
-                    const bf16x8 bf = *reinterpret_cast<const bf16x8*>(&bs[s][k + (lane >> 5)][wc + j * 32 + (lane & 31)][0]);
-#pragma unroll
-                    for (int i = 0; i < mi; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[i], bf, acc[i][j], 0, 0, 0);
-                }
+        int64_t k = 0;
+        for (; k + 1 < whole; k += 2) {
+            step(0, k);
+            step(1, k + 1);
         }
+        if (k < whole) step(0, k);
+    }
+    if (r_begin + whole * kRows < r_end) {
+        __syncthreads();
+        load_rest(r_begin + whole * kRows);
+        stage(0, 0);
+        __syncthreads();
+        product(0, 0);
+        product(0, 2);
     }
     float* out = a.partial + (int64_t(slab) * tiles + tile) * (BM * BN);
 #pragma unroll
@@ -260,10 +331,12 @@ __global__ void __launch_bounds__(kBlock, 2) ckpt_gram_kernel(const GramArgs a) 
                 out[(wr + i * 32 + 8 * (k >> 2) + 4 * (lane >> 5) + (k & 3)) * BN + wc + j * 32 + (lane & 31)] = acc[i][j][k];
 }
 
-// the slabs' partial sums, in order; 64 results to a workgroup, its four waves take a quarter of the slabs each
-__global__ void __launch_bounds__(kBlock) ckpt_gram_join(const float* __restrict__ partial, int32_t slabs, int32_t tiles_m, int32_t tiles_n,
+// the slabs' partial sums, in order; 64 results to a workgroup, its waves take a share of the slabs each
+constexpr int kJoin = 1024;
+__global__ void __launch_bounds__(kJoin) ckpt_gram_join(const float* __restrict__ partial, int32_t slabs, int32_t tiles_m, int32_t tiles_n,
                                                          int32_t bm, int32_t bn, int32_t m, int32_t n, float* __restrict__ out) {
-    __shared__ double part[kBlock / 64][64];
+    constexpr int waves = kJoin / 64;
+    __shared__ double part[waves][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int32_t e = int32_t(blockIdx.x) * 64 + lane;
     const bool in = e < m * n;
@@ -273,41 +346,45 @@ __global__ void __launch_bounds__(kBlock) ckpt_gram_join(const float* __restrict
         const int32_t tile = i / bm + (j / bn) * tiles_m, ii = i % bm;
         const float* p = partial + int64_t(tile) * bm * bn + ((ii & 3) * (bm / 4) + (ii >> 2)) * bn + j % bn;
         const int64_t step = int64_t(tiles_m) * tiles_n * bm * bn;
-        const int32_t s0 = int32_t(int64_t(slabs) * wave / 4), s1 = int32_t(int64_t(slabs) * (wave + 1) / 4);
+        const int32_t s0 = slabs * wave / waves, s1 = slabs * (wave + 1) / waves;
 #pragma unroll 8
         for (int32_t s = s0; s < s1; ++s) sum += double(p[s * step]);
     }
     part[wave][lane] = sum;
     __syncthreads();
-    if (wave == 0 && in) out[e] = float(((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane]);
+    if (wave == 0 && in) {
+        for (int w = 1; w < waves; ++w) sum += part[w][lane];
+        out[e] = float(sum);
+    }
 }
 
 struct GramPlan {
-    int32_t bm, bn, kt, tiles_m, tiles_n, slabs;
+    int32_t bm, bn, tiles_m, tiles_n, slabs;
     int64_t slab_rows;
 };
 
-// Tile: the smallest that covers the result where it is small, 256 x 128 where it is not.  Slabs: two workgroups for each CU.
+// Tile: 64 or 128 rows of a small result, 384 where that saves a second conversion of G, else 256; 32, 64 or 128 columns.
 GramPlan gram_plan(int64_t rows, int32_t m, int32_t n) {
     GramPlan p;
     const int32_t mp = (m + 31) & ~31;
-    p.bm = mp <= 128 || (mp > 256 && mp <= 384) ? 128 : 256;
+    p.bm = mp <= 64 && n <= 64 ? 64 : mp <= 128 ? 128 : mp <= 256 || n <= 64 || mp > 768 ? 256 : 384;
     p.bn = n <= 32 ? 32 : n <= 64 ? 64 : 128;
-    p.kt = p.bm == 256 ? 32 : 64;
     p.tiles_m = (mp + p.bm - 1) / p.bm;
     p.tiles_n = (n + p.bn - 1) / p.bn;
-    const int64_t want = (512 + p.tiles_m * p.tiles_n - 1) / (p.tiles_m * p.tiles_n);
-    int64_t each = (rows + want - 1) / want;
-    each = (each + p.kt - 1) / p.kt * p.kt;
-    p.slab_rows = each < p.kt ? p.kt : each;
+    // workgroups that a CU holds at once (registers and LDS of the tile); no more, or the last ones run alone
+    const int32_t held = p.bm == 384 ? 1 : p.bn == 128 ? 2 : p.bm == 256 ? (p.bn == 32 ? 3 : 2) : 4;
+    const int64_t want = (256 * held) / (p.tiles_m * p.tiles_n);
+    int64_t each = want > 1 ? (rows + want - 1) / want : rows;
+    each = (each + kRows - 1) / kRows * kRows;
+    p.slab_rows = each < kLeast ? kLeast : each;
     p.slabs = int32_t((rows + p.slab_rows - 1) / p.slab_rows);
     return p;
 }
 
-template <int BM, int BN, int KT>
+template <int BM, int BN, int WM, int WN>
 void launch_gram(const GramArgs& a, hipStream_t stream) {
     const unsigned blocks = unsigned((a.slabs + 7) / 8 * 8) * unsigned(a.tiles_m * a.tiles_n);
-    ckpt_gram_kernel<BM, BN, KT><<<blocks, kBlock, 0, stream>>>(a);
+    ckpt_gram_kernel<BM, BN, WM, WN><<<blocks, 64 * WM * WN, 0, stream>>>(a);
 }
 
 unsigned grid_of(int64_t items) {
@@ -377,7 +454,7 @@ extern "C" int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t
     if (int rc = check_checkpoint(codes, scales, n_rows, m)) return rc;
     MH_REQUIRE(n >= 1 && int64_t(m) * n <= (int64_t(1) << 30), "m=%d n=%d", m, n);
     MH_REQUIRE(out, "null pointer");
-    MH_REQUIRE(ldg >= 0 && img >= 0, "negative stride");
+    MH_REQUIRE(ldg >= 0 && img >= 0 && ldg <= (1 << 24) && img <= (int64_t(1) << 40), "row stride of G: %lld", (long long)ldg);
     GramArgs a{};
     if (n_rows > 0) {
         MH_REQUIRE(G && workspace, "null pointer");
@@ -389,18 +466,20 @@ extern "C" int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t
     a.slab_rows = p.slab_rows; a.m = m; a.mp = (m + 31) & ~31; a.n = n; a.slabs = p.slabs; a.tiles_m = p.tiles_m; a.tiles_n = p.tiles_n;
     a.partial = static_cast<float*>(workspace);
     if (n_rows > 0) {
-        const int key = p.bm * 1000 + p.bn;
-        switch (key) {
-            case 128032: launch_gram<128, 32, 64>(a, stream); break;
-            case 128064: launch_gram<128, 64, 64>(a, stream); break;
-            case 128128: launch_gram<128, 128, 64>(a, stream); break;
-            case 256032: launch_gram<256, 32, 32>(a, stream); break;
-            case 256064: launch_gram<256, 64, 32>(a, stream); break;
-            default: launch_gram<256, 128, 32>(a, stream); break;
+        switch (p.bm * 1000 + p.bn) {
+            case 64032: launch_gram<64, 32, 2, 1>(a, stream); break;
+            case 64064: launch_gram<64, 64, 2, 1>(a, stream); break;
+            case 128032: launch_gram<128, 32, 2, 1>(a, stream); break;
+            case 128064: launch_gram<128, 64, 2, 1>(a, stream); break;
+            case 128128: launch_gram<128, 128, 2, 2>(a, stream); break;
+            case 256032: launch_gram<256, 32, 4, 1>(a, stream); break;
+            case 256064: launch_gram<256, 64, 4, 1>(a, stream); break;
+            case 256128: launch_gram<256, 128, 2, 2>(a, stream); break;
+            default: launch_gram<384, 128, 4, 2>(a, stream); break;
         }
         MH_LAUNCH_CHECK("ckpt_gram");
     }
-    ckpt_gram_join<<<unsigned((int64_t(m) * n + 63) / 64), kBlock, 0, stream>>>(a.partial, a.slabs, a.tiles_m, a.tiles_n, p.bm, p.bn, m, n, out);
+    ckpt_gram_join<<<unsigned((int64_t(m) * n + 63) / 64), kJoin, 0, stream>>>(a.partial, a.slabs, a.tiles_m, a.tiles_n, p.bm, p.bn, m, n, out);
     MH_LAUNCH_CHECK("ckpt_gram_join");
     return MH_OK;
 }
