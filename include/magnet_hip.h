@@ -319,6 +319,7 @@ int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t n_rows, in
  *     Y = gamma (X - m) / sqrt(v + eps) + beta on both parts  [relu: both parts times (Re Y >= 0)]
  * gamma, beta: float[F] or NULL (1, 0).  Rows behind the last graph are written as zeros; a graph may be empty.
  * stats: float[n_graphs * groups * MH_NORM_STATS], for the backward pass.  mask_out: uint8 [n_rows][F] or NULL, the gate.
+ * codes_out, scales_out: a checkpoint of X as mh_ckpt_store makes it, or both NULL.
  *   mh_group_norm_bwd  dX, dgamma, dbeta (each may be NULL) from the gradient G of Y.  The input is X, or, where codes is not
  *                      NULL, its checkpoint (mh_ckpt_store), with the gate from `mask` when relu (X is not read then).
  * workspace: mh_group_norm_workspace_bytes, 8-byte aligned, contents irrelevant before and after.  Statistics and sums are
@@ -328,7 +329,8 @@ int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t n_rows, in
 size_t mh_group_norm_workspace_bytes(int64_t n_rows, int32_t n_graphs, int32_t F, int32_t groups);
 int mh_group_norm(const float* X, int64_t ld, int64_t im, int64_t n_rows, int32_t F, int32_t groups, const int32_t* graph_ptr,
                   int32_t n_graphs, float eps, const float* gamma, const float* beta, int relu, float* Y, int64_t ldy, int64_t imy,
-                  uint8_t* mask_out, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+                  uint8_t* mask_out, uint8_t* codes_out, uint8_t* scales_out, float* stats, void* workspace,
+                  size_t workspace_bytes, void* stream);
 int mh_group_norm_bwd(const float* X, int64_t ld, int64_t im, const uint8_t* codes, const uint8_t* scales, const uint8_t* mask,
                       int64_t n_rows, int32_t F, int32_t groups, const int32_t* graph_ptr, int32_t n_graphs, const float* stats,
                       const float* gamma, const float* beta, int relu, const float* G, int64_t ldg, int64_t img, float* dX,

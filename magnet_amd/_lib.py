@@ -101,7 +101,7 @@ def _load():
     lib.mh_group_norm_workspace_bytes.restype = sz
     lib.mh_group_norm_workspace_bytes.argtypes = [i64, i32, i32, i32]
     lib.mh_group_norm.restype = C.c_int
-    lib.mh_group_norm.argtypes = [vp, i64, i64, i64, i32, i32, vp, i32, f32, vp, vp, C.c_int, vp, i64, i64, vp, vp, vp, sz, vp]
+    lib.mh_group_norm.argtypes = [vp, i64, i64, i64, i32, i32, vp, i32, f32, vp, vp, C.c_int, vp, i64, i64, vp, vp, vp, vp, vp, sz, vp]
     lib.mh_group_norm_bwd.restype = C.c_int
     lib.mh_group_norm_bwd.argtypes = [vp, i64, i64, vp, vp, vp, i64, i32, i32, vp, i32, vp, vp, vp, C.c_int, vp, i64, i64, vp, i64, i64,
                                       vp, vp, vp, sz, vp]

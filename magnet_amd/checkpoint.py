@@ -40,6 +40,12 @@ class Checkpoint8:
             self.columns *= v
 
     @staticmethod
+    def memory(n, m, device):
+        """Uninitialised (codes, scales) of a checkpoint of [n, 2, m]."""
+        codes = torch.empty((2 * n, -(-m // BLOCK) * BLOCK), dtype=torch.uint8, device=device)
+        return codes, torch.empty((codes.size(1) // BLOCK, -(-2 * n // 8) * 8), dtype=torch.uint8, device=device)
+
+    @staticmethod
     def store(x):
         """Checkpoint of x.  Any row and part strides, the columns contiguous; a block [N, 2, K + 1, F] must be contiguous
         in its last two dimensions."""
@@ -51,8 +57,7 @@ class Checkpoint8:
             x = x.flatten(2)
         x = contiguous_columns(x)
         n, _, m = x.shape
-        codes = torch.empty((2 * n, -(-m // BLOCK) * BLOCK), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((codes.size(1) // BLOCK, -(-2 * n // 8) * 8), dtype=torch.uint8, device=x.device)
+        codes, scales = Checkpoint8.memory(n, m, x.device)
         ops.ckpt_store(x, codes, scales)
         return Checkpoint8(codes, scales, shape)
 

@@ -473,18 +473,25 @@ void check_groups(int64_t f, int64_t groups) {
 
 // stats [n_graphs, groups, MH_NORM_STATS], for the backward pass
 Tensor group_norm(const Tensor& X, int64_t groups, const OptTensor& graph_ptr, double eps, const OptTensor& gamma, const OptTensor& beta,
-                  bool relu, Tensor& out, const OptTensor& mask) {
+                  bool relu, Tensor& out, const OptTensor& mask, const OptTensor& codes, const OptTensor& scales) {
     const c10::DeviceGuard guard(X.device());
     Planar x = planar(X, "X"), y = planar(out, "out");
     same_device(X, out, "out");
     TORCH_CHECK(y.n == x.n && y.f == x.f, "out has shape ", out.sizes(), ", expected ", X.sizes());
     check_groups(x.f, groups);
     Batch b = batch_of(graph_ptr, X, x.n);
+    uint8_t *c = nullptr, *s = nullptr;
+    if (codes.has_value() && codes->defined()) {
+        TORCH_CHECK(scales.has_value() && scales->defined(), "codes without scales");
+        same_device(X, *codes, "codes");
+        Held h = held(*codes, *scales, x.n, x.f);
+        c = h.codes; s = h.scales;
+    }
     Tensor stats = at::empty({b.n, groups, MH_NORM_STATS}, X.options());
     Tensor ws = norm_workspace(X, x.n, b.n, x.f, groups);
     check_rc(mh_group_norm(x.p, x.ld, x.im, x.n, int32_t(x.f), int32_t(groups), b.ptr, b.n, float(eps), channels_of(gamma, "weight", X, x.f),
                            channels_of(beta, "bias", X, x.f), relu ? 1 : 0, y.p, y.ld, y.im, mask_of(mask, x.n, x.f),
-                           stats.data_ptr<float>(), ws.data_ptr(), size_t(ws.numel()) * sizeof(double), stream_of(X)), "group_norm");
+                           c, s, stats.data_ptr<float>(), ws.data_ptr(), size_t(ws.numel()) * sizeof(double), stream_of(X)), "group_norm");
     return stats;
 }
 
@@ -799,7 +806,7 @@ TORCH_LIBRARY(magnet, m) {
     m.def("ckpt_restore(Tensor codes, Tensor scales, Tensor(a!) out) -> ()");
     m.def("ckpt_gram(Tensor codes, Tensor scales, int m, Tensor G) -> Tensor");
     m.def("group_norm(Tensor X, int groups, Tensor? graph_ptr, float eps, Tensor? gamma, Tensor? beta, bool relu, Tensor(a!) out, "
-          "Tensor(b!)? mask) -> Tensor");
+          "Tensor(b!)? mask, Tensor(c!)? codes, Tensor(d!)? scales) -> Tensor");
     m.def("group_norm_bwd(Tensor? X, Tensor? codes, Tensor? scales, Tensor? mask, Tensor G, int groups, Tensor? graph_ptr, "
           "Tensor stats, Tensor? gamma, Tensor? beta, bool relu, Tensor(a!)? dX, Tensor(b!)? dgamma, Tensor(c!)? dbeta) -> ()");
     m.def("class_logprobs(Tensor scores, Tensor? labels, int ignore, Tensor(a!)? logprob, Tensor(b!) entropy, Tensor(c!)? stat, "

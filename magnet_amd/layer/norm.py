@@ -23,14 +23,13 @@ class _GroupNormFn(torch.autograd.Function):
         n, _, f = x.shape
         xc = contiguous_columns(x)
         out = _alloc_out(n, f, next_terms, x.device)
-        held = Checkpoint8.store(xc) if keep == 8 else None
-        mask = torch.empty((n, f), dtype=torch.uint8, device=x.device) if held is not None and relu else None
-        stats = ops.group_norm(xc, groups, graph_ptr, eps, weight, bias, relu, out, mask)
+        codes = scales = mask = None
+        if keep == 8:                                  # the checkpoint is made by the pass that reads x anyway
+            codes, scales = Checkpoint8.memory(n, f, x.device)
+            mask = torch.empty((n, f), dtype=torch.uint8, device=x.device) if relu else None
+        stats = ops.group_norm(xc, groups, graph_ptr, eps, weight, bias, relu, out, mask, codes, scales)
         ctx.groups, ctx.relu = groups, relu
-        if held is None:
-            ctx.save_for_backward(x, None, None, None, weight, bias, graph_ptr, stats)
-        else:
-            ctx.save_for_backward(None, held.codes, held.scales, mask, weight, bias, graph_ptr, stats)
+        ctx.save_for_backward(x if codes is None else None, codes, scales, mask, weight, bias, graph_ptr, stats)
         return out
 
     @staticmethod

@@ -45,8 +45,8 @@ def test_group_norm_entry_points_refuse_bad_arguments():
     lib = _lib()
     big = 1 << 40
 
-    def norm(x=FAKE, ld=16, im=8, n=10, f=8, groups=2, ptr=None, graphs=1, y=FAKE, ldy=16, imy=8, ws=FAKE, ws_bytes=big, stats=FAKE):
-        return lib.mh_group_norm(x, ld, im, n, f, groups, ptr, graphs, 1e-5, None, None, 0, y, ldy, imy, None, stats, ws, ws_bytes, None)
+    def norm(x=FAKE, ld=16, im=8, n=10, f=8, groups=2, ptr=None, graphs=1, y=FAKE, ldy=16, imy=8, ws=FAKE, ws_bytes=big, stats=FAKE, codes=None):
+        return lib.mh_group_norm(x, ld, im, n, f, groups, ptr, graphs, 1e-5, None, None, 0, y, ldy, imy, None, codes, None, stats, ws, ws_bytes, None)
 
     _says(lib, norm(groups=3), -1, b'divide')
     _says(lib, norm(groups=0), -1, b'divide')
@@ -57,6 +57,7 @@ def test_group_norm_entry_points_refuse_bad_arguments():
     _says(lib, norm(x=None), -1, b'null')
     _says(lib, norm(stats=None), -1, b'null')
     _says(lib, norm(ldy=4), -1, b'stride')
+    _says(lib, norm(codes=FAKE), -1, b'null')                                      # codes without scales
     _says(lib, norm(ws_bytes=8), -4, b'workspace')
     _says(lib, norm(ws=ODD), -1, b'aligned')
     assert norm(x=None, n=0, y=None, graphs=0, ws=None, stats=None) == 0

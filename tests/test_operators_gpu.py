@@ -689,6 +689,7 @@ def test_network_with_norms_against_64_bits(layer, graphs):
     lab = torch.randint(0, 4, (1, n), generator=_gen(3))
     loss, _ = class_nll(net.scores(net.trunk(real.to(DEV), imag.to(DEV))), lab.to(DEV))
     loss.backward()
+    loss = loss.detach()
     z, params = _plain_trunk(net, lap, torch.complex(real.double(), imag.double()), ptr)
     feats = torch.cat((z.real, z.imag), 1)
     scores = feats @ params['Conv.weight'].squeeze(-1).t() + params['Conv.bias']
@@ -696,7 +697,7 @@ def test_network_with_norms_against_64_bits(layer, graphs):
     want.backward()
     # the framework's bar for float32 forward and backward results, 1e-5 of a tensor's largest value; a gate on the border of 0
     # may open one value of float32's accuracy on the other side
-    assert abs(float(loss) - float(want)) <= 1e-5 * abs(float(want))
+    assert abs(float(loss) - want.item()) <= 1e-5 * abs(want.item())
     for k, p in net.named_parameters():
         ref = params[k].grad
         assert float((p.grad.double().cpu() - ref).abs().max()) <= 2e-5 * float(ref.abs().max()) + 1e-9, k
