@@ -4,7 +4,7 @@
 // For a row x[0..C):  m = max x,  s = sum e^(x-m),  w = sum e^(x-m) (x-m)
 //     log p_c = (x_c - m) - log s          entropy H = log s - w / s
 //     d log p_y / d x_c = [c = y] - p_c    d H / d x_c = -p_c (log p_c + H)
-// (m, s, w) of two parts of a row join as  m' = max(m1, m2), s' = sum e^(mi-m') si, w' = sum e^(mi-m') (wi + si (mi-m')).
+// (m, s, w) of a part of a row go to a larger maximum m' as  s' = e^(m-m') s, w' = e^(m-m') (w + s (m - m')), and then add.
 // All of it in 32 bits whatever the type of the scores, the sum over rows of the loss in 64.
 //
 // A row belongs to a group of `1 << ll` lanes, 64 >> ll rows to a wavefront.  Row-major scores: the lanes of a group are
@@ -47,33 +47,116 @@ __device__ inline float key_value(uint32_t k) {
 // (value, class) as one integer: the larger value first, then the lower class
 __device__ inline uint64_t candidate(float x, uint32_t c) { return (uint64_t(order_key(x)) << 32) | uint32_t(~c); }
 
+// e^x to a few units in the last place for the weights of a row: x <= 0, and what |x| costs its accuracy its weight forgives
+__device__ inline float weight(float x) { return __expf(x); }
+
+// (m, s, w) of a part of a row
 struct Soft {
     float m = -INFINITY, s = 0.0f, w = 0.0f;
+    // to a maximum that is no less; a part without weight takes its infinite exponent with it, a NaN in s stays
+    __device__ void raise(float to) {
+        const float d = m - to, e = s == 0.0f ? 0.0f : weight(d);
+        w = e == 0.0f ? 0.0f : e * (w + s * d);
+        s = e * s;
+        m = to;
+    }
+    __device__ void join(Soft o) {
+        const float to = fmaxf(m, o.m);
+        raise(to);
+        o.raise(to);
+        s += o.s;
+        w += o.w;
+    }
+    // values below or at the maximum
+    __device__ void add(const float (&x)[kPer]) {
+        const float from = m == -INFINITY ? 0.0f : m;          // nothing but -inf: the sums stay 0 (and NaN stays NaN)
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const float t = x[j] - from, e = weight(t);
+            s += e;
+            w += e == 0.0f ? 0.0f : e * t;
+        }
+    }
 };
 
-__device__ inline void join(Soft& a, const Soft& b) {
-    const float m = fmaxf(a.m, b.m);
-    const float da = a.m - m, db = b.m - m;
-    const float ea = a.s == 0.0f ? 0.0f : expf(da), eb = b.s == 0.0f ? 0.0f : expf(db);
-    // a part that has no weight left next to the other takes its (possibly infinite) exponent with it
-    const float wa = ea == 0.0f ? 0.0f : ea * (a.w + a.s * da), wb = eb == 0.0f ? 0.0f : eb * (b.w + b.s * db);
-    a.s = ea * a.s + eb * b.s;                                      // a NaN in s stays, whatever its part's maximum
-    a.w = wa + wb;
-    a.m = m;
+__device__ inline float largest(const float (&x)[kPer]) {
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < kPer; ++j) m = fmaxf(m, x[j]);
+    return m == m ? m : -INFINITY;                              // nothing but NaN
 }
 
-__device__ inline Soft of_values(const float (&x)[kPer]) {
-    Soft r;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) r.m = fmaxf(r.m, x[j]);
-    const float m = r.m == -INFINITY ? 0.0f : r.m;     // nothing but -inf: the sums stay 0 (and NaN stays NaN)
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const float t = x[j] - m, e = expf(t);
-        r.s += e;
-        r.w += e == 0.0f ? 0.0f : e * t;
+// Sum and maximum over the lanes of a group: over a whole wavefront by data-parallel moves (six instructions, no LDS), else by
+// xor shuffles.
+template <int CTRL, int ROWS>
+__device__ inline uint32_t moved(uint32_t v, uint32_t idle) { return uint32_t(__builtin_amdgcn_update_dpp(int(idle), int(v), CTRL, ROWS, 0xf, false)); }
+#define MH_WAVE_FOLD(v, idle, OP)                                                                                        \
+    v = OP(v, (moved<0x111, 0xf>(v, idle))); v = OP(v, (moved<0x112, 0xf>(v, idle))); v = OP(v, (moved<0x114, 0xf>(v, idle))); \
+    v = OP(v, (moved<0x118, 0xf>(v, idle))); v = OP(v, (moved<0x142, 0xa>(v, idle))); v = OP(v, (moved<0x143, 0xc>(v, idle))); \
+    v = uint32_t(__builtin_amdgcn_readlane(int(v), 63))
+__device__ inline uint32_t op_add(uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }
+__device__ inline uint32_t op_fmax(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+__device__ inline uint32_t op_umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+struct Group {
+    int lanes, near;                        // lanes of a row, distance of two neighbours
+    __device__ float sum(float x) const {
+        if (lanes == 64) {
+            uint32_t v = __float_as_uint(x);
+            MH_WAVE_FOLD(v, 0u, op_add);
+            return __uint_as_float(v);
+        }
+        for (int o = near; o < near * lanes; o <<= 1) x += __shfl_xor(x, o);
+        return x;
     }
-    return r;
+    __device__ float max(float x) const {
+        if (lanes == 64) {
+            uint32_t v = __float_as_uint(x);
+            MH_WAVE_FOLD(v, 0xff800000u, op_fmax);
+            return __uint_as_float(v);
+        }
+        for (int o = near; o < near * lanes; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+        return x;
+    }
+    __device__ uint64_t max(uint64_t x) const {
+        for (int o = near; o < near * lanes; o <<= 1) {
+            const uint64_t other = __shfl_xor(static_cast<unsigned long long>(x), o);
+            x = other > x ? other : x;
+        }
+        return x;
+    }
+};
+
+// The best candidate of a row whose keys all lie in registers (class j * lanes + l, key 0: none), taken out of them.  Over a whole
+// wavefront the key is found by a maximum and its first class by ballots, without a 64-bit comparison for each step.
+__device__ inline uint64_t take_best(uint32_t (&key)[kPer], const Group& g, int l) {
+    uint32_t best = key[0];
+    if (g.lanes == 64) {
+#pragma unroll
+        for (int j = 1; j < kPer; ++j) best = op_umax(best, key[j]);
+        MH_WAVE_FOLD(best, 0u, op_umax);
+        uint64_t got = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const uint64_t who = got == 0 ? __ballot(key[j] == best) : 0;
+            if (who) {
+                const int first = __ffsll(static_cast<unsigned long long>(who)) - 1;
+                got = (uint64_t(best) << 32) | uint32_t(~uint32_t(j * 64 + first));
+                if (l == first) key[j] = 0;
+            }
+        }
+        return got;
+    }
+    int at = 0;
+#pragma unroll
+    for (int j = 1; j < kPer; ++j) {
+        at = key[j] > best ? j : at;
+        best = op_umax(best, key[j]);
+    }
+    const uint64_t mine = (uint64_t(best) << 32) | uint32_t(~uint32_t(at * g.lanes + l)), top = g.max(mine);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) key[j] = mine == top && j == at ? 0u : key[j];
+    return top;
 }
 
 template <int N>
@@ -123,27 +206,31 @@ __device__ inline void place(const ScoreArgs& a, int64_t row, int64_t& b, int64_
     i = row - b * a.inner;
 }
 
-template <class T, int TOPN, bool NLL, bool JOIN>
+// ONE: a row's classes fit its lanes' registers, and the best are taken from there.  Else a lane keeps a list of its TOPN best.
+template <class T, int TOPN, bool NLL, bool ONE, bool JOIN>
 __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int rows_of_wave = 64 >> a.ll, lanes = 1 << a.ll;
     const int r = a.by_class ? lane & (rows_of_wave - 1) : lane >> a.ll;
     const int l = a.by_class ? lane >> (6 - a.ll) : lane & (lanes - 1);
-    const int near = a.by_class ? rows_of_wave : 1;                 // distance of two neighbours of a group
+    const Group group{lanes, a.by_class ? rows_of_wave : 1};
     const int waves = kBlock / 64;
     const int64_t step = int64_t(rows_of_wave) * (JOIN ? 1 : waves) * gridDim.x;
     const int64_t first = (int64_t(blockIdx.x) * (JOIN ? 1 : waves) + (JOIN ? 0 : wave)) * rows_of_wave;
     double sum = 0.0;
     int32_t used = 0, hits = 0;
-    // every lane of a wave makes the same number of turns: a row past the end only takes part in the shuffles
+    // every lane of a wave makes the same number of turns: a row past the end only takes part in the exchanges
     for (int64_t row0 = first; row0 < a.rows; row0 += step) {
         const int64_t row = row0 + r;
         const bool live = row < a.rows;
         int64_t b = 0, i = 0;
         if (live) place(a, row, b, i);
         const T* x = static_cast<const T*>(a.x) + b * a.sb + i * a.sn;
+        const bool writes = live && l == 0;
+        const int64_t label = writes && a.labels ? a.labels[row] : 0;
         Soft acc;
         TopList<TOPN> best;
+        uint32_t key[kPer];
         for (int32_t c0 = JOIN ? wave * kPer * lanes : 0; c0 < a.classes; c0 += kPer * lanes * (JOIN ? waves : 1)) {
             float v[kPer];
 #pragma unroll
@@ -151,20 +238,20 @@ __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
                 const int32_t c = c0 + j * lanes + l;
                 v[j] = live && c < a.classes ? to_f(x[c * a.sc]) : -INFINITY;
             }
-            join(acc, of_values(v));
-            if (TOPN > 0) {
+            if (ONE) acc.m = group.max(largest(v));
+            else acc.raise(fmaxf(acc.m, largest(v)));
+            acc.add(v);
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    const int32_t c = c0 + j * lanes + l;
-                    if (c < a.classes) best.add(candidate(v[j], uint32_t(c)));
-                }
+            for (int j = 0; j < kPer; ++j) {
+                const int32_t c = c0 + j * lanes + l;
+                if (ONE) key[j] = c < a.classes ? order_key(v[j]) : 0u;
+                else if (TOPN > 0 && c < a.classes) best.add(candidate(v[j], uint32_t(c)));
             }
+            if (ONE) break;
         }
-        for (int o = near; o < near * lanes; o <<= 1) {
-            Soft other;
-            other.m = __shfl_xor(acc.m, o); other.s = __shfl_xor(acc.s, o); other.w = __shfl_xor(acc.w, o);
-            join(acc, other);
-        }
+        if (!ONE) acc.raise(group.max(acc.m));
+        acc.s = group.sum(acc.s);
+        acc.w = group.sum(acc.w);
         if (JOIN) {
             __shared__ float soft[kBlock / 64][64][3];
             __shared__ uint64_t lists[TOPN > 0 ? kBlock / 64 : 1][64][TOPN > 0 ? TOPN : 1];
@@ -177,52 +264,43 @@ __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
                 for (int v = 1; v < waves; ++v) {
                     Soft other;
                     other.m = soft[v][lane][0]; other.s = soft[v][lane][1]; other.w = soft[v][lane][2];
-                    join(acc, other);
+                    acc.join(other);
 #pragma unroll
                     for (int t = 0; t < TOPN; ++t) best.add(lists[v][lane][t]);
                 }
             }
         }
         if (JOIN && wave != 0) continue;                           // waves leave the turn together: row0 is the workgroup's
+        auto next_best = [&]() {
+            if (ONE) return take_best(key, group, l);
+            const uint64_t top = group.max(best.v[0]);
+            if (best.v[0] == top) best.pop();                      // one lane holds it: a candidate carries its class
+            return top;
+        };
         const float log_s = logf(acc.s);
-        const bool writes = live && l == 0;
         float lp = 0.0f;
-        int64_t label = 0;
-        bool counted = false;
-        if (writes && a.labels) {
-            label = a.labels[row];
-            counted = label != a.ignore;
-            if (counted) lp = label >= 0 && label < a.classes ? (to_f(x[label * a.sc]) - acc.m) - log_s : NAN;
-        }
+        const bool counted = writes && a.labels && label != a.ignore;
+        if (counted) lp = label >= 0 && label < a.classes ? (to_f(x[label * a.sc]) - acc.m) - log_s : NAN;
         if (writes && a.stat) a.stat[row] = make_float2(acc.m, log_s);
         if (NLL) {
-            uint64_t top1 = best.v[0];
-            for (int o = near; o < near * lanes; o <<= 1) {
-                const uint64_t other = __shfl_xor(static_cast<unsigned long long>(top1), o);
-                top1 = other > top1 ? other : top1;
-            }
+            const uint64_t top = next_best();
             if (counted) {
                 sum += double(lp);
                 ++used;
-                hits += int64_t(uint32_t(~uint32_t(top1))) == label;
+                hits += int64_t(uint32_t(~uint32_t(top))) == label;
             }
         } else {
             if (writes) {
                 if (a.logprob) a.logprob[row] = lp;
                 a.entropy[row] = log_s - acc.w / acc.s;
             }
-            if (TOPN > 0) {
+            if (ONE || TOPN > 0) {
                 for (int t = 0; t < a.top; ++t) {
-                    uint64_t top1 = best.v[0];
-                    for (int o = near; o < near * lanes; o <<= 1) {
-                        const uint64_t other = __shfl_xor(static_cast<unsigned long long>(top1), o);
-                        top1 = other > top1 ? other : top1;
-                    }
-                    if (best.v[0] == top1) best.pop();             // one lane holds it: a candidate carries its class
+                    const uint64_t top = next_best();
                     if (writes) {
                         const int64_t at = b * a.tb + t * a.tk + i * a.tn;
-                        a.top_idx[at] = int64_t(uint32_t(~uint32_t(top1)));
-                        a.top_lp[at] = (key_value(uint32_t(top1 >> 32)) - acc.m) - log_s;
+                        a.top_idx[at] = int64_t(uint32_t(~uint32_t(top)));
+                        a.top_lp[at] = (key_value(uint32_t(top >> 32)) - acc.m) - log_s;
                     }
                 }
             }
@@ -277,7 +355,50 @@ struct GradArgs {
     int64_t tb, tk, tn;
 };
 
-// d x_c = [c = y] g_y + sum_t [c = i_t] g_t - p_c (g_y + sum_t g_t) - p_c (log p_c + H) g_H
+// d x_c = [c = y] g_y + sum_t [c = i_t] g_t - p_c (g_y + sum_t g_t) - p_c (log p_c + H) g_H: what it takes of a row
+struct RowGrad {
+    int64_t at;                             // of the alternatives
+    int32_t label;                          // -1: none
+    float gy, gh, h, all, m, log_s;
+    bool any;
+};
+
+template <bool NLL>
+__device__ inline RowGrad row_grad(const GradArgs& a, int64_t row, int64_t b, int64_t i, float scale) {
+    RowGrad r;
+    const int64_t label = a.labels ? a.labels[row] : a.ignore;
+    const bool counted = a.labels && label != a.ignore, inside = label >= 0 && label < a.classes;
+    r.label = counted && inside ? int32_t(label) : -1;
+    r.gy = !counted ? 0.0f : !inside ? NAN : NLL ? scale : a.g_lp ? a.g_lp[row * a.g_lp_s] : 0.0f;      // NaN as its log probability
+    r.gh = !NLL && a.g_h ? a.g_h[row * a.g_h_s] : 0.0f;
+    r.h = !NLL && a.g_h ? a.entropy[row] : 0.0f;
+    r.all = r.gy;
+    r.any = r.gy != 0.0f || r.gh != 0.0f;
+    r.at = b * a.tb + i * a.tn;
+    if (!NLL && a.g_top)
+        for (int t = 0; t < a.top; ++t) {
+            const float g = a.g_top[r.at + t * a.tk];
+            r.all += g;
+            r.any |= g != 0.0f;
+        }
+    const float2 st = a.stat[row];
+    r.m = st.x;
+    r.log_s = st.y;
+    return r;
+}
+
+template <bool NLL>
+__device__ inline float score_grad(const GradArgs& a, const RowGrad& r, float x, int32_t c) {
+    if (!r.any) return 0.0f;                // a row no gradient reaches stays clean whatever it holds
+    const float lp = (x - r.m) - r.log_s, p = weight(lp);
+    float g = (c == r.label ? r.gy : 0.0f) - p * r.all;
+    if (!NLL && a.g_h) g -= p == 0.0f ? 0.0f : p * (lp + r.h) * r.gh;
+    if (!NLL && a.g_top)
+        for (int t = 0; t < a.top; ++t)
+            if (a.top_idx[r.at + t * a.tk] == c) g += a.g_top[r.at + t * a.tk];
+    return g;
+}
+
 template <class T, bool NLL>
 __global__ void __launch_bounds__(kBlock) score_grads(const GradArgs a) {
     const int lane = threadIdx.x & 63;
@@ -291,22 +412,7 @@ __global__ void __launch_bounds__(kBlock) score_grads(const GradArgs a) {
         const int64_t b = a.rows == a.inner ? 0 : row / a.inner, i = row - b * a.inner;
         const T* x = static_cast<const T*>(a.x) + b * a.sb + i * a.sn;
         T* d = static_cast<T*>(a.d) + b * a.db + i * a.dn;
-        const int64_t label = a.labels ? a.labels[row] : a.ignore;
-        const bool counted = a.labels && label != a.ignore;
-        float gy = !counted ? 0.0f : NLL ? scale : a.g_lp ? a.g_lp[row * a.g_lp_s] : 0.0f;
-        if (counted && (label < 0 || label >= a.classes)) gy = NAN;      // as its log probability
-        const float gh = !NLL && a.g_h ? a.g_h[row * a.g_h_s] : 0.0f;
-        const float h = !NLL && a.g_h ? a.entropy[row] : 0.0f;
-        float all = gy;
-        bool any = gy != 0.0f || gh != 0.0f;
-        const int64_t at = b * a.tb + i * a.tn;
-        if (!NLL && a.g_top)
-            for (int t = 0; t < a.top; ++t) {
-                const float g = a.g_top[at + t * a.tk];
-                all += g;
-                any |= g != 0.0f;
-            }
-        const float2 st = a.stat[row];
+        const RowGrad g = row_grad<NLL>(a, row, b, i, scale);
         for (int32_t c0 = l; c0 < a.classes; c0 += kPer * lanes) {
             float v[kPer];
 #pragma unroll
@@ -317,26 +423,49 @@ __global__ void __launch_bounds__(kBlock) score_grads(const GradArgs a) {
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
                 const int32_t c = c0 + j * lanes;
-                if (c < a.classes) {
-                    float g = 0.0f;                                  // a row no gradient reaches stays clean whatever it holds
-                    if (any) {
-                        const float lp = (v[j] - st.x) - st.y, p = expf(lp);
-                        g = (c == label && counted ? gy : 0.0f) - p * all;
-                        if (!NLL && a.g_h) g -= p == 0.0f ? 0.0f : p * (lp + h) * gh;
-                        if (!NLL && a.g_top)
-                            for (int t = 0; t < a.top; ++t)
-                                if (a.top_idx[at + t * a.tk] == c) g += a.g_top[at + t * a.tk];
-                    }
-                    d[c * a.dc] = from_f<T>(g);
-                }
+                if (c < a.classes) d[c * a.dc] = from_f<T>(score_grad<NLL>(a, g, v[j], c));
             }
         }
     }
 }
 
+// Dense rows one behind the other, at least as many classes as 16 bytes hold: the gradient is elementwise once (m, log s, H) are
+// known, so a thread takes 16 bytes wherever they fall in at most two rows, and a row's length and alignment do not matter.
+template <class T, bool NLL>
+__global__ void __launch_bounds__(kBlock) score_grads_flat(const GradArgs a) {
+    constexpr int E = 16 / sizeof(T);
+    struct alignas(16) Pack { T v[E]; };
+    const int64_t total = a.rows * a.classes, first = (int64_t(blockIdx.x) * kBlock + threadIdx.x) * E;
+    if (first >= total) return;
+    const float scale = NLL ? -a.g_loss[0] * a.inv_count[0] : 0.0f;
+    const int64_t row = total <= UINT32_MAX ? int64_t(uint32_t(first) / uint32_t(a.classes)) : first / a.classes;
+    const int32_t c0 = int32_t(first - row * a.classes);
+    const T* x = static_cast<const T*>(a.x) + first;
+    T* d = static_cast<T*>(a.d) + first;
+    const bool whole = first + E <= total;
+    Pack in;
+    if (whole) in = *reinterpret_cast<const Pack*>(x);
+    else
+        for (int e = 0; e < E; ++e)
+            if (first + e < total) in.v[e] = x[e];
+    const RowGrad g0 = row_grad<NLL>(a, row, 0, row, scale);
+    RowGrad g1 = g0;
+    if (c0 + E > a.classes && row + 1 < a.rows) g1 = row_grad<NLL>(a, row + 1, 0, row + 1, scale);
+    Pack out;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const bool next = c0 + e >= a.classes;
+        out.v[e] = from_f<T>(score_grad<NLL>(a, next ? g1 : g0, to_f(in.v[e]), next ? c0 + e - a.classes : c0 + e));
+    }
+    if (whole) *reinterpret_cast<Pack*>(d) = out;
+    else
+        for (int e = 0; e < E; ++e)
+            if (first + e < total) d[e] = out.v[e];
+}
+
 struct Shape {
     int ll, by_class;
-    bool join;
+    bool join, one;
     unsigned blocks;
 };
 
@@ -350,6 +479,7 @@ Shape shape_of(int64_t rows, int32_t classes, int64_t sc, int64_t sn, bool can_j
     s.ll = 0;
     while (s.ll < 6 && (int64_t(kPer) << s.ll) < classes && (!s.by_class || (rows << s.ll) < fill)) ++s.ll;
     const int64_t tiles = (rows + (64 >> s.ll) - 1) / (64 >> s.ll);
+    s.one = (int64_t(kPer) << s.ll) >= classes;
     s.join = can_join && s.ll == 6 && tiles < 1024 && classes > 2 * kPer * 64;
     const int64_t b = s.join ? tiles : (tiles + kBlock / 64 - 1) / (kBlock / 64);
     s.blocks = unsigned(b < 1 ? 1 : b > kMostBlocks ? kMostBlocks : b);
@@ -358,16 +488,37 @@ Shape shape_of(int64_t rows, int32_t classes, int64_t sc, int64_t sn, bool can_j
 
 template <class T, int TOPN, bool NLL>
 void launch_rows(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
-    if (s.join) score_rows<T, TOPN, NLL, true><<<s.blocks, kBlock, 0, stream>>>(a);
-    else score_rows<T, TOPN, NLL, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    if (s.join) score_rows<T, TOPN, NLL, false, true><<<s.blocks, kBlock, 0, stream>>>(a);
+    else score_rows<T, TOPN, NLL, false, false><<<s.blocks, kBlock, 0, stream>>>(a);
 }
 
 template <class T>
 void launch_report(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
-    if (a.top == 0) launch_rows<T, 0, false>(a, s, stream);
+    if (s.one) score_rows<T, 0, false, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    else if (a.top == 0) launch_rows<T, 0, false>(a, s, stream);
     else if (a.top <= 2) launch_rows<T, 2, false>(a, s, stream);
     else if (a.top <= 8) launch_rows<T, 8, false>(a, s, stream);
     else launch_rows<T, kMostTop, false>(a, s, stream);
+}
+
+template <class T, bool NLL>
+void launch_grads(GradArgs a, hipStream_t stream) {
+    constexpr int E = 16 / sizeof(T);
+    const int64_t total = a.rows * a.classes, blocks = (total + int64_t(kBlock) * E - 1) / (int64_t(kBlock) * E);
+    const bool dense = a.rows == a.inner && a.sc == 1 && a.dc == 1 && a.sn == a.classes && a.dn == a.classes && a.classes >= E;
+    if (dense && blocks <= INT32_MAX && mh_aligned16(a.x) && mh_aligned16(a.d)) {
+        score_grads_flat<T, NLL><<<unsigned(blocks), kBlock, 0, stream>>>(a);
+        return;
+    }
+    const Shape s = shape_of(a.rows, a.classes, a.sc, a.sn, false);
+    a.ll = s.ll; a.by_class = s.by_class;
+    score_grads<T, NLL><<<s.blocks, kBlock, 0, stream>>>(a);
+}
+
+template <class T>
+void launch_nll(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
+    if (s.one) score_rows<T, 0, true, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    else launch_rows<T, 1, true>(a, s, stream);
 }
 
 int check_scores(const void* x, int dtype, int64_t n_batch, int64_t n_inner, int32_t classes, int64_t sb, int64_t sc, int64_t sn) {
@@ -423,11 +574,9 @@ extern "C" int mh_class_logprobs_bwd(const void* scores, int dtype, int64_t n_ba
     a.classes = classes; a.labels = g_logprob ? labels : nullptr; a.ignore = ignore; a.stat = reinterpret_cast<const float2*>(stat);
     a.entropy = entropy; a.g_lp = g_logprob; a.g_lp_s = g_logprob_stride; a.g_h = g_entropy; a.g_h_s = g_entropy_stride;
     a.g_top = top ? g_top : nullptr; a.top_idx = top_index; a.top = top; a.tb = tb; a.tk = tk; a.tn = tn;
-    const Shape s = shape_of(rows, classes, sc, sn, false);
-    a.ll = s.ll; a.by_class = s.by_class;
-    if (dtype == 0) score_grads<float, false><<<s.blocks, kBlock, 0, stream>>>(a);
-    else if (dtype == 1) score_grads<__hip_bfloat16, false><<<s.blocks, kBlock, 0, stream>>>(a);
-    else score_grads<__half, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    if (dtype == 0) launch_grads<float, false>(a, stream);
+    else if (dtype == 1) launch_grads<__hip_bfloat16, false>(a, stream);
+    else launch_grads<__half, false>(a, stream);
     MH_LAUNCH_CHECK("class_logprobs_bwd");
     return MH_OK;
 }
@@ -452,9 +601,9 @@ extern "C" int mh_class_nll(const void* scores, int dtype, int64_t n_batch, int6
         const Shape s = shape_of(rows, classes, sc, sn, true);
         a.ll = s.ll; a.by_class = s.by_class;
         blocks = s.blocks;
-        if (dtype == 0) launch_rows<float, 1, true>(a, s, stream);
-        else if (dtype == 1) launch_rows<__hip_bfloat16, 1, true>(a, s, stream);
-        else launch_rows<__half, 1, true>(a, s, stream);
+        if (dtype == 0) launch_nll<float>(a, s, stream);
+        else if (dtype == 1) launch_nll<__hip_bfloat16>(a, s, stream);
+        else launch_nll<__half>(a, s, stream);
         MH_LAUNCH_CHECK("class_nll");
     }
     nll_finish<<<1, kBlock, 0, stream>>>(a.partial, int(blocks), loss, accuracy, inv_count);
@@ -476,11 +625,9 @@ extern "C" int mh_class_nll_bwd(const void* scores, int dtype, int64_t n_batch, 
     a.x = scores; a.d = d_scores; a.rows = rows; a.inner = n_inner; a.sb = sb; a.sc = sc; a.sn = sn; a.db = db; a.dc = dc; a.dn = dn;
     a.classes = classes; a.labels = labels; a.ignore = ignore; a.stat = reinterpret_cast<const float2*>(stat);
     a.g_loss = g_loss; a.inv_count = inv_count;
-    const Shape s = shape_of(rows, classes, sc, sn, false);
-    a.ll = s.ll; a.by_class = s.by_class;
-    if (dtype == 0) score_grads<float, true><<<s.blocks, kBlock, 0, stream>>>(a);
-    else if (dtype == 1) score_grads<__hip_bfloat16, true><<<s.blocks, kBlock, 0, stream>>>(a);
-    else score_grads<__half, true><<<s.blocks, kBlock, 0, stream>>>(a);
+    if (dtype == 0) launch_grads<float, true>(a, stream);
+    else if (dtype == 1) launch_grads<__hip_bfloat16, true>(a, stream);
+    else launch_grads<__half, true>(a, stream);
     MH_LAUNCH_CHECK("class_nll_bwd");
     return MH_OK;
 }
