@@ -147,8 +147,8 @@ lib = _load()
 OPS = ['cspmm', 'cspmm_noalloc', 'plan_build', 'cheb_terms_', 'clenshaw', 'lap_build', 'lap_block_count',
        'lap_block_fill', 'pack', 'unpack',
        'gather_rows', 'scatter_rows', 'bias_relu_', 'relu_bwd_', 'relu_bwd_out',
-       'ckpt_store', 'ckpt_restore', 'ckpt_gram', 'group_norm', 'group_norm_bwd',
-       'class_logprobs', 'class_logprobs_bwd', 'class_nll', 'class_nll_bwd', 'halo_plan', 'powerlaw_edges', 'stream_read',
+       'ckpt_store', 'ckpt_restore', 'ckpt_gram', 'group_norm', 'class_logprobs',
+       'class_nll', 'halo_plan', 'powerlaw_edges', 'stream_read',
        'set_spmm_grid_cap', 'noalloc_init', 'exchange_new_id', 'exchange_create', 'exchange_begin', 'exchange_end',
        'exchange_all_gather', 'exchange_destroy', 'version']
 

@@ -24,8 +24,10 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kPer = 8;                    // classes a lane holds at a time
+constexpr int kMore = 24;                  // the same where a row of more than 64 classes fits a few lanes that way
 constexpr int kMostTop = 16;
-constexpr unsigned kMostBlocks = 2048;     // 8 workgroups of 4 waves per CU
+constexpr unsigned kMostSums = 2048;       // workgroups that leave a partial sum of the loss: 8 of 4 waves for each CU
+constexpr unsigned kMostBlocks = 1u << 20;
 
 __device__ inline float to_f(float v) { return v; }
 __device__ inline float to_f(__hip_bfloat16 v) { return __bfloat162float(v); }
@@ -68,10 +70,11 @@ struct Soft {
         w += o.w;
     }
     // values below or at the maximum
-    __device__ void add(const float (&x)[kPer]) {
+    template <int P>
+    __device__ void add(const float (&x)[P]) {
         const float from = m == -INFINITY ? 0.0f : m;          // nothing but -inf: the sums stay 0 (and NaN stays NaN)
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
+        for (int j = 0; j < P; ++j) {
             const float t = x[j] - from, e = weight(t);
             s += e;
             w += e == 0.0f ? 0.0f : e * t;
@@ -79,45 +82,41 @@ struct Soft {
     }
 };
 
-__device__ inline float largest(const float (&x)[kPer]) {
+template <int P>
+__device__ inline float largest(const float (&x)[P]) {
     float m = x[0];
 #pragma unroll
-    for (int j = 1; j < kPer; ++j) m = fmaxf(m, x[j]);
+    for (int j = 1; j < P; ++j) m = fmaxf(m, x[j]);
     return m == m ? m : -INFINITY;                              // nothing but NaN
 }
 
-// Sum and maximum over the lanes of a group: over a whole wavefront by data-parallel moves (six instructions, no LDS), else by
-// xor shuffles.
+// Sum, maximum and minimum over the lanes of a group: over a whole wavefront or 16 neighbours by data-parallel moves (six or four
+// instructions, no LDS), else by xor shuffles.
 template <int CTRL, int ROWS>
 __device__ inline uint32_t moved(uint32_t v, uint32_t idle) { return uint32_t(__builtin_amdgcn_update_dpp(int(idle), int(v), CTRL, ROWS, 0xf, false)); }
-#define MH_WAVE_FOLD(v, idle, OP)                                                                                        \
-    v = OP(v, (moved<0x111, 0xf>(v, idle))); v = OP(v, (moved<0x112, 0xf>(v, idle))); v = OP(v, (moved<0x114, 0xf>(v, idle))); \
-    v = OP(v, (moved<0x118, 0xf>(v, idle))); v = OP(v, (moved<0x142, 0xa>(v, idle))); v = OP(v, (moved<0x143, 0xc>(v, idle))); \
-    v = uint32_t(__builtin_amdgcn_readlane(int(v), 63))
-__device__ inline uint32_t op_add(uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }
-__device__ inline uint32_t op_fmax(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
-__device__ inline uint32_t op_umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+struct Add { static __device__ uint32_t of(uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); } };
+struct MaxF { static __device__ uint32_t of(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); } };
+struct MaxU { static __device__ uint32_t of(uint32_t a, uint32_t b) { return a > b ? a : b; } };
+struct MinU { static __device__ uint32_t of(uint32_t a, uint32_t b) { return a < b ? a : b; } };
 
 struct Group {
     int lanes, near;                        // lanes of a row, distance of two neighbours
-    __device__ float sum(float x) const {
-        if (lanes == 64) {
-            uint32_t v = __float_as_uint(x);
-            MH_WAVE_FOLD(v, 0u, op_add);
-            return __uint_as_float(v);
+    template <class Op>
+    __device__ uint32_t fold(uint32_t v, uint32_t idle) const {
+        if (lanes == 64) {                  // shift by 1, 2, 4, 8 inside rows of 16, then across them; lane 63 has it all
+            v = Op::of(v, moved<0x111, 0xf>(v, idle)); v = Op::of(v, moved<0x112, 0xf>(v, idle)); v = Op::of(v, moved<0x114, 0xf>(v, idle));
+            v = Op::of(v, moved<0x118, 0xf>(v, idle)); v = Op::of(v, moved<0x142, 0xa>(v, idle)); v = Op::of(v, moved<0x143, 0xc>(v, idle));
+            return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
         }
-        for (int o = near; o < near * lanes; o <<= 1) x += __shfl_xor(x, o);
-        return x;
-    }
-    __device__ float max(float x) const {
-        if (lanes == 64) {
-            uint32_t v = __float_as_uint(x);
-            MH_WAVE_FOLD(v, 0xff800000u, op_fmax);
-            return __uint_as_float(v);
+        if (lanes == 16 && near == 1) {     // rotate by 8, 4, 2, 1
+            v = Op::of(v, moved<0x128, 0xf>(v, idle)); v = Op::of(v, moved<0x124, 0xf>(v, idle));
+            v = Op::of(v, moved<0x122, 0xf>(v, idle)); return Op::of(v, moved<0x121, 0xf>(v, idle));
         }
-        for (int o = near; o < near * lanes; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
-        return x;
+        for (int o = near; o < near * lanes; o <<= 1) v = Op::of(v, uint32_t(__shfl_xor(int(v), o)));
+        return v;
     }
+    __device__ float sum(float x) const { return __uint_as_float(fold<Add>(__float_as_uint(x), 0u)); }
+    __device__ float max(float x) const { return __uint_as_float(fold<MaxF>(__float_as_uint(x), 0xff800000u)); }
     __device__ uint64_t max(uint64_t x) const {
         for (int o = near; o < near * lanes; o <<= 1) {
             const uint64_t other = __shfl_xor(static_cast<unsigned long long>(x), o);
@@ -127,36 +126,23 @@ struct Group {
     }
 };
 
-// The best candidate of a row whose keys all lie in registers (class j * lanes + l, key 0: none), taken out of them.  Over a whole
-// wavefront the key is found by a maximum and its first class by ballots, without a 64-bit comparison for each step.
-__device__ inline uint64_t take_best(uint32_t (&key)[kPer], const Group& g, int l) {
+// The best candidate of a row whose keys all lie in registers (class j * lanes + l, key 0: none), taken out of them: the largest key,
+// then the first class that has it
+template <int P>
+__device__ inline uint64_t take_best(uint32_t (&key)[P], const Group& g, int l) {
     uint32_t best = key[0];
-    if (g.lanes == 64) {
-#pragma unroll
-        for (int j = 1; j < kPer; ++j) best = op_umax(best, key[j]);
-        MH_WAVE_FOLD(best, 0u, op_umax);
-        uint64_t got = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const uint64_t who = got == 0 ? __ballot(key[j] == best) : 0;
-            if (who) {
-                const int first = __ffsll(static_cast<unsigned long long>(who)) - 1;
-                got = (uint64_t(best) << 32) | uint32_t(~uint32_t(j * 64 + first));
-                if (l == first) key[j] = 0;
-            }
-        }
-        return got;
-    }
     int at = 0;
 #pragma unroll
-    for (int j = 1; j < kPer; ++j) {
+    for (int j = 1; j < P; ++j) {
         at = key[j] > best ? j : at;
-        best = op_umax(best, key[j]);
+        best = MaxU::of(best, key[j]);
     }
-    const uint64_t mine = (uint64_t(best) << 32) | uint32_t(~uint32_t(at * g.lanes + l)), top = g.max(mine);
+    const uint32_t top = g.fold<MaxU>(best, 0u), mine = best == top ? uint32_t(at * g.lanes + l) : ~0u;
+    const uint32_t c = g.fold<MinU>(mine, ~0u);
+    at = mine == c ? at : -1;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) key[j] = mine == top && j == at ? 0u : key[j];
-    return top;
+    for (int j = 0; j < P; ++j) key[j] = j == at ? 0u : key[j];
+    return (uint64_t(top) << 32) | uint32_t(~c);
 }
 
 template <int N>
@@ -207,7 +193,7 @@ __device__ inline void place(const ScoreArgs& a, int64_t row, int64_t& b, int64_
 }
 
 // ONE: a row's classes fit its lanes' registers, and the best are taken from there.  Else a lane keeps a list of its TOPN best.
-template <class T, int TOPN, bool NLL, bool ONE, bool JOIN>
+template <class T, int P, int TOPN, bool NLL, bool ONE, bool JOIN>
 __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int rows_of_wave = 64 >> a.ll, lanes = 1 << a.ll;
@@ -230,22 +216,25 @@ __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
         const int64_t label = writes && a.labels ? a.labels[row] : 0;
         Soft acc;
         TopList<TOPN> best;
-        uint32_t key[kPer];
-        for (int32_t c0 = JOIN ? wave * kPer * lanes : 0; c0 < a.classes; c0 += kPer * lanes * (JOIN ? waves : 1)) {
-            float v[kPer];
+        uint32_t key[P];
+        float of_label = 0.0f;
+        for (int32_t c0 = JOIN ? wave * P * lanes : 0; c0 < a.classes; c0 += P * lanes * (JOIN ? waves : 1)) {
+            float v[P];
+            const T* at = x + (c0 + l) * a.sc;
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const int32_t c = c0 + j * lanes + l;
-                v[j] = live && c < a.classes ? to_f(x[c * a.sc]) : -INFINITY;
+            for (int j = 0; j < P; ++j) {
+                v[j] = live && c0 + j * lanes + l < a.classes ? to_f(*at) : -INFINITY;
+                at += lanes * a.sc;
             }
             if (ONE) acc.m = group.max(largest(v));
             else acc.raise(fmaxf(acc.m, largest(v)));
             acc.add(v);
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
+            for (int j = 0; j < P; ++j) {
                 const int32_t c = c0 + j * lanes + l;
                 if (ONE) key[j] = c < a.classes ? order_key(v[j]) : 0u;
                 else if (TOPN > 0 && c < a.classes) best.add(candidate(v[j], uint32_t(c)));
+                if (ONE && P == kPer) of_label = c == label ? v[j] : of_label;
             }
             if (ONE) break;
         }
@@ -280,7 +269,11 @@ __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
         const float log_s = logf(acc.s);
         float lp = 0.0f;
         const bool counted = writes && a.labels && label != a.ignore;
-        if (counted) lp = label >= 0 && label < a.classes ? (to_f(x[label * a.sc]) - acc.m) - log_s : NAN;
+        if (counted) {
+            const bool inside = label >= 0 && label < a.classes;
+            if (inside && !(ONE && P == kPer && lanes == 1)) of_label = to_f(x[label * a.sc]);
+            lp = inside ? (of_label - acc.m) - log_s : NAN;
+        }
         if (writes && a.stat) a.stat[row] = make_float2(acc.m, log_s);
         if (NLL) {
             const uint64_t top = next_best();
@@ -295,10 +288,10 @@ __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
                 a.entropy[row] = log_s - acc.w / acc.s;
             }
             if (ONE || TOPN > 0) {
-                for (int t = 0; t < a.top; ++t) {
+                int64_t at = b * a.tb + i * a.tn;
+                for (int t = 0; t < a.top; ++t, at += a.tk) {
                     const uint64_t top = next_best();
                     if (writes) {
-                        const int64_t at = b * a.tb + t * a.tk + i * a.tn;
                         a.top_idx[at] = int64_t(uint32_t(~uint32_t(top)));
                         a.top_lp[at] = (key_value(uint32_t(top >> 32)) - acc.m) - log_s;
                     }
@@ -464,37 +457,39 @@ __global__ void __launch_bounds__(kBlock) score_grads_flat(const GradArgs a) {
 }
 
 struct Shape {
-    int ll, by_class;
+    int ll, by_class, per;
     bool join, one;
     unsigned blocks;
 };
 
-// Lanes of a row.  Row-major: as many as hold the row at kPer classes each (fewer joins, whole lines read once), at most a
-// wavefront.  Class-major: one, unless there are too few rows to fill the GPU.  A workgroup joins on its rows when even
-// whole wavefronts per row are too few for the GPU and every wave gets classes.
-Shape shape_of(int64_t rows, int32_t classes, int64_t sc, int64_t sn, bool can_join) {
+// Lanes of a row.  Row-major: as many as hold the row at kPer classes each, past 64 classes at kMore each but 16 at least (60k x 349
+// with 5 alternatives: 80 us on 64 lanes of 8, WIDE us on 16 of 24).  Class-major: one, unless there are too few rows to fill the GPU.
+// A workgroup joins on its rows when even whole wavefronts per row are too few for the GPU and every wave gets classes.
+Shape shape_of(int64_t rows, int32_t classes, int64_t sc, int64_t sn, bool can_join, unsigned most) {
     Shape s;
     s.by_class = sc > sn && sn != 0;
     const int64_t fill = int64_t(256) * 8 * 64;            // two waves per SIMD
-    s.ll = 0;
-    while (s.ll < 6 && (int64_t(kPer) << s.ll) < classes && (!s.by_class || (rows << s.ll) < fill)) ++s.ll;
+    s.per = !s.by_class && classes > 64 && classes <= kMore * 64 ? kMore : kPer;
+    s.ll = s.per == kMore ? 4 : 0;
+    while (s.ll < 6 && (int64_t(s.per) << s.ll) < classes && (!s.by_class || (rows << s.ll) < fill)) ++s.ll;
     const int64_t tiles = (rows + (64 >> s.ll) - 1) / (64 >> s.ll);
-    s.one = (int64_t(kPer) << s.ll) >= classes;
-    s.join = can_join && s.ll == 6 && tiles < 1024 && classes > 2 * kPer * 64;
+    s.one = (int64_t(s.per) << s.ll) >= classes;
+    s.join = can_join && s.ll == 6 && tiles < 1024 && !s.one && classes > 2 * kPer * 64;
     const int64_t b = s.join ? tiles : (tiles + kBlock / 64 - 1) / (kBlock / 64);
-    s.blocks = unsigned(b < 1 ? 1 : b > kMostBlocks ? kMostBlocks : b);
+    s.blocks = unsigned(b < 1 ? 1 : b > most ? most : b);
     return s;
 }
 
 template <class T, int TOPN, bool NLL>
 void launch_rows(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
-    if (s.join) score_rows<T, TOPN, NLL, false, true><<<s.blocks, kBlock, 0, stream>>>(a);
-    else score_rows<T, TOPN, NLL, false, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    if (s.join) score_rows<T, kPer, TOPN, NLL, false, true><<<s.blocks, kBlock, 0, stream>>>(a);
+    else score_rows<T, kPer, TOPN, NLL, false, false><<<s.blocks, kBlock, 0, stream>>>(a);
 }
 
 template <class T>
 void launch_report(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
-    if (s.one) score_rows<T, 0, false, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    if (s.one && s.per == kMore) score_rows<T, kMore, 0, false, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    else if (s.one) score_rows<T, kPer, 0, false, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
     else if (a.top == 0) launch_rows<T, 0, false>(a, s, stream);
     else if (a.top <= 2) launch_rows<T, 2, false>(a, s, stream);
     else if (a.top <= 8) launch_rows<T, 8, false>(a, s, stream);
@@ -510,14 +505,15 @@ void launch_grads(GradArgs a, hipStream_t stream) {
         score_grads_flat<T, NLL><<<unsigned(blocks), kBlock, 0, stream>>>(a);
         return;
     }
-    const Shape s = shape_of(a.rows, a.classes, a.sc, a.sn, false);
+    const Shape s = shape_of(a.rows, a.classes, a.sc, a.sn, false, kMostBlocks);
     a.ll = s.ll; a.by_class = s.by_class;
     score_grads<T, NLL><<<s.blocks, kBlock, 0, stream>>>(a);
 }
 
 template <class T>
 void launch_nll(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
-    if (s.one) score_rows<T, 0, true, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    if (s.one && s.per == kMore) score_rows<T, kMore, 0, true, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    else if (s.one) score_rows<T, kPer, 0, true, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
     else launch_rows<T, 1, true>(a, s, stream);
 }
 
@@ -547,7 +543,7 @@ extern "C" int mh_class_logprobs(const void* scores, int dtype, int64_t n_batch,
     a.labels = labels; a.ignore = ignore; a.stat = reinterpret_cast<float2*>(stat);
     a.logprob = labels ? logprob : nullptr; a.entropy = entropy; a.top_lp = top_logprob; a.top_idx = top_index; a.top = top;
     a.tb = tb; a.tk = tk; a.tn = tn;
-    const Shape s = shape_of(rows, classes, sc, sn, true);
+    const Shape s = shape_of(rows, classes, sc, sn, true, kMostBlocks);
     a.ll = s.ll; a.by_class = s.by_class;
     if (dtype == 0) launch_report<float>(a, s, stream);
     else if (dtype == 1) launch_report<__hip_bfloat16>(a, s, stream);
@@ -581,7 +577,7 @@ extern "C" int mh_class_logprobs_bwd(const void* scores, int dtype, int64_t n_ba
     return MH_OK;
 }
 
-extern "C" size_t mh_class_nll_workspace_bytes(void) { return size_t(kMostBlocks) * 3 * sizeof(double); }
+extern "C" size_t mh_class_nll_workspace_bytes(void) { return size_t(kMostSums) * 3 * sizeof(double); }
 
 extern "C" int mh_class_nll(const void* scores, int dtype, int64_t n_batch, int64_t n_inner, int32_t classes, int64_t sb, int64_t sc,
                             int64_t sn, const int64_t* labels, int64_t ignore, float* stat, float* loss, float* accuracy,
@@ -598,7 +594,7 @@ extern "C" int mh_class_nll(const void* scores, int dtype, int64_t n_batch, int6
     if (rows > 0) {
         a.x = scores; a.rows = rows; a.inner = n_inner; a.sb = sb; a.sc = sc; a.sn = sn; a.classes = classes;
         a.labels = labels; a.ignore = ignore; a.stat = reinterpret_cast<float2*>(stat);
-        const Shape s = shape_of(rows, classes, sc, sn, true);
+        const Shape s = shape_of(rows, classes, sc, sn, true, kMostSums);
         a.ll = s.ll; a.by_class = s.by_class;
         blocks = s.blocks;
         if (dtype == 0) launch_nll<float>(a, s, stream);

@@ -5,6 +5,9 @@
 // device pointers, strides and the CURRENT torch stream of the operand's device, forwards them to
 // the corresponding mh_* entry point and turns a non-zero return code into a RuntimeError that
 // carries mh_last_error().  torch is the allocator and the stream owner; no arithmetic happens here.
+// The operators with gradients (group_norm, class_logprobs, class_nll) are autograd functions of torch here rather than in
+// Python: a training step on a small graph is bound by what the host does for each call (loss, accuracy and gradient of 2500 x 5
+// scores: 88 us through Python functions).
 //
 // The reference reaches this path through Python calls into torch.sparse
 // (reference src/layer/sparse_magnet.py:8-18,50-72) and scipy (src/utils/hermitian.py:136-168);
@@ -17,6 +20,8 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include "../../include/magnet_hip.h"
@@ -471,19 +476,14 @@ void check_groups(int64_t f, int64_t groups) {
     TORCH_CHECK(f >= 1 && f <= (1 << 20) && groups >= 1 && f % groups == 0, f, " channels do not divide into ", groups, " groups");
 }
 
-// stats [n_graphs, groups, MH_NORM_STATS], for the backward pass
-Tensor group_norm(const Tensor& X, int64_t groups, const OptTensor& graph_ptr, double eps, const OptTensor& gamma, const OptTensor& beta,
-                  bool relu, Tensor& out, const OptTensor& mask, const OptTensor& codes, const OptTensor& scales) {
-    const c10::DeviceGuard guard(X.device());
-    Planar x = planar(X, "X"), y = planar(out, "out");
-    same_device(X, out, "out");
-    TORCH_CHECK(y.n == x.n && y.f == x.f, "out has shape ", out.sizes(), ", expected ", X.sizes());
+// the result, and stats [n_graphs, groups, MH_NORM_STATS] for the backward pass
+Tensor norm_forward(const Tensor& X, int64_t groups, const OptTensor& graph_ptr, double eps, const OptTensor& gamma, const OptTensor& beta,
+                    bool relu, Tensor& out, const OptTensor& mask, const OptTensor& codes, const OptTensor& scales) {
+    Planar x = planar(X, "x"), y = planar(out, "out");
     check_groups(x.f, groups);
     Batch b = batch_of(graph_ptr, X, x.n);
     uint8_t *c = nullptr, *s = nullptr;
-    if (codes.has_value() && codes->defined()) {
-        TORCH_CHECK(scales.has_value() && scales->defined(), "codes without scales");
-        same_device(X, *codes, "codes");
+    if (codes.has_value()) {
         Held h = held(*codes, *scales, x.n, x.f);
         c = h.codes; s = h.scales;
     }
@@ -495,33 +495,92 @@ Tensor group_norm(const Tensor& X, int64_t groups, const OptTensor& graph_ptr, d
     return stats;
 }
 
-void group_norm_bwd(const OptTensor& X, const OptTensor& codes, const OptTensor& scales, const OptTensor& mask, const Tensor& G,
-                    int64_t groups, const OptTensor& graph_ptr, const Tensor& stats, const OptTensor& gamma, const OptTensor& beta,
-                    bool relu, const OptTensor& dX, const OptTensor& dgamma, const OptTensor& dbeta) {
-    const c10::DeviceGuard guard(G.device());
-    Planar g = planar(G, "G");
-    check_groups(g.f, groups);
-    Planar x = planar_opt(X, "X", g.n, g.f), dx = planar_opt(dX, "dX", g.n, g.f);
+void norm_backward(const OptTensor& X, const OptTensor& codes, const OptTensor& scales, const OptTensor& mask, const Tensor& G,
+                   int64_t groups, const OptTensor& graph_ptr, const Tensor& stats, const OptTensor& gamma, const OptTensor& beta,
+                   bool relu, const OptTensor& dX, const OptTensor& dgamma, const OptTensor& dbeta) {
+    Planar g = planar(G, "gradient");
+    Planar x = planar_opt(X, "x", g.n, g.f), dx = planar_opt(dX, "dx", g.n, g.f);
     uint8_t *c = nullptr, *s = nullptr;
     if (codes.has_value() && codes->defined()) {
-        TORCH_CHECK(scales.has_value() && scales->defined(), "codes without scales");
-        same_device(G, *codes, "codes");
         Held h = held(*codes, *scales, g.n, g.f);
         c = h.codes; s = h.scales;
-    } else {
-        TORCH_CHECK(X.has_value() && X->defined(), "neither the input nor its checkpoint is given");
-        same_device(G, *X, "X");
     }
     Batch b = batch_of(graph_ptr, G, g.n);
-    need_cuda(stats, "stats");
-    TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == int64_t(b.n) * groups * MH_NORM_STATS,
-                "stats must be the tensor group_norm returned");
     Tensor ws = norm_workspace(G, g.n, b.n, g.f, groups);
     auto out = [&](const OptTensor& t, const char* name) { return const_cast<float*>(channels_of(t, name, G, g.f)); };
     check_rc(mh_group_norm_bwd(x.p, x.ld, x.im, c, s, mask_of(mask, g.n, g.f), g.n, int32_t(g.f), int32_t(groups), b.ptr, b.n,
                                stats.data_ptr<float>(), channels_of(gamma, "weight", G, g.f), channels_of(beta, "bias", G, g.f),
-                               relu ? 1 : 0, g.p, g.ld, g.im, dx.p, dx.ld, dx.im, out(dgamma, "dgamma"), out(dbeta, "dbeta"), ws.data_ptr(),
+                               relu ? 1 : 0, g.p, g.ld, g.im, dx.p, dx.ld, dx.im, out(dgamma, "dweight"), out(dbeta, "dbias"), ws.data_ptr(),
                                size_t(ws.numel()) * sizeof(double), stream_of(G)), "group_norm_bwd");
+}
+
+// [N, 2, F] with its columns contiguous; an empty tensor counts as contiguous at any strides
+Tensor columns(const Tensor& t) {
+    if (t.dim() != 3 || t.size(2) <= 1 || t.stride(2) == 1) return t;
+    return t.numel() ? t.contiguous() : at::empty(t.sizes(), t.options());
+}
+
+OptTensor some(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// gradients that are not differentiable themselves: asked to be (create_graph), they raise when it comes to that
+variable_list once(variable_list grads, const char* what) {
+    if (!at::GradMode::is_enabled()) return grads;
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string("the gradient of ") + what + " cannot be differentiated again",
+                                                                 int64_t(grads.size()));
+    return (*error)(std::move(grads));
+}
+
+struct GroupNorm : public torch::autograd::Function<GroupNorm> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups,
+                          const OptTensor& graph_ptr, double eps, bool relu, int64_t bits, int64_t next_terms) {
+        const c10::DeviceGuard guard(x.device());
+        Tensor xc = columns(x);
+        const int64_t n = x.size(0), f = x.size(2);
+        Tensor out = next_terms > 1 ? at::empty({n, 2, next_terms, f}, x.options()).select(2, 0) : at::empty({n, 2, f}, x.options());
+        Tensor codes, scales, mask;
+        if (bits == 8) {                               // the checkpoint is made by the pass that reads x anyway
+            auto bytes = x.options().dtype(at::kByte);
+            codes = at::empty({2 * n, (f + 31) / 32 * 32}, bytes);
+            scales = at::empty({(f + 31) / 32, (2 * n + 7) / 8 * 8}, bytes);
+            if (relu) mask = at::empty({n, f}, bytes);
+        }
+        Tensor stats = norm_forward(xc, groups, graph_ptr, eps, weight, bias, relu, out, some(mask), some(codes), some(scales));
+        ctx->save_for_backward({bits == 8 ? Tensor() : x, codes, scales, mask, weight.value_or(Tensor()), bias.value_or(Tensor()),
+                                graph_ptr.value_or(Tensor()), stats});
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["relu"] = relu;
+        return out;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list s = ctx->get_saved_variables();
+        const Tensor &x = s[0], &weight = s[4], &bias = s[5];
+        Tensor g = columns(grads[0]);
+        const c10::DeviceGuard guard(g.device());
+        Tensor dx, dw, db;
+        if (ctx->needs_input_grad(0)) dx = at::empty(g.sizes(), g.options());
+        size_t edge = 1;                               // the operands that are there, in order
+        if (weight.defined() && ctx->needs_input_grad(edge++)) dw = at::empty_like(weight);
+        if (bias.defined() && ctx->needs_input_grad(edge++)) db = at::empty_like(bias);
+        norm_backward(x.defined() ? OptTensor(columns(x)) : OptTensor(), some(s[1]), some(s[2]), some(s[3]), g, ctx->saved_data["groups"].toInt(),
+                      some(s[6]), s[7], some(weight), some(bias), ctx->saved_data["relu"].toBool(), some(dx), some(dw), some(db));
+        variable_list out = once({dx, dw, db}, "group_norm");
+        out.resize(9);
+        return out;
+    }
+};
+
+Tensor group_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, const OptTensor& graph_ptr, double eps,
+                  bool relu, int64_t bits, int64_t next_terms) {
+    need_cuda(x, "x");
+    TORCH_CHECK(x.dim() == 3 && x.size(1) == 2, "x must be row-planar [N, 2, F], got ", x.sizes());
+    TORCH_CHECK(bits == 8 || bits == 32, "checkpoint_bits is 8 or 32, got ", bits);
+    auto differentiated = [](const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); };
+    const bool wanted = at::GradMode::is_enabled() && (x.requires_grad() || differentiated(weight) || differentiated(bias));
+    return GroupNorm::apply(x, weight, bias, groups, graph_ptr, eps, relu, wanted ? bits : 32, next_terms);
 }
 
 // ---- class scores ------------------------------------------------------------------------------
@@ -546,116 +605,157 @@ Scores scores_of(const Tensor& t, const char* name) {
     return s;
 }
 
-const int64_t* labels_of(const OptTensor& t, const Tensor& scores, int64_t rows) {
-    if (!t.has_value() || !t->defined()) return nullptr;
-    need_cuda(*t, "labels");
-    same_device(scores, *t, "labels");
-    TORCH_CHECK(t->scalar_type() == at::kLong && t->is_contiguous() && t->numel() == rows, "labels must be contiguous int64 with ", rows,
-                " entries, got ", t->scalar_type(), " ", t->sizes());
-    return t->data_ptr<int64_t>();
-}
-
-float* rows_of(const OptTensor& t, const char* name, const Tensor& scores, int64_t n) {
-    if (!t.has_value() || !t->defined()) return nullptr;
-    need_cuda(*t, name);
-    same_device(scores, *t, name);
-    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == n, name, " must be contiguous float32 with ", n, " entries");
-    return t->data_ptr<float>();
-}
-
-// gradient of one value per row: contiguous, or one value expanded over all rows
-std::pair<const float*, int64_t> row_grad(const OptTensor& t, const char* name, const Tensor& scores, int64_t n) {
-    if (!t.has_value() || !t->defined()) return {nullptr, 0};
-    need_cuda(*t, name);
-    same_device(scores, *t, name);
-    TORCH_CHECK(t->scalar_type() == at::kFloat && t->numel() == n, name, " must be float32 with ", n, " entries");
-    bool expanded = true;
-    for (int64_t d = 0; d < t->dim(); ++d) expanded = expanded && (t->size(d) <= 1 || t->stride(d) == 0);
-    TORCH_CHECK(expanded || t->is_contiguous(), name, " must be contiguous or one value expanded");
-    return {t->data_ptr<float>(), expanded ? 0 : 1};
-}
-
-struct Top {
-    int32_t k = 0;
-    int64_t tb = 0, tk = 0, tn = 0;
+// a gradient of one value per row, readable with stride 1, or 0 where it is one value expanded (that of a sum or a mean)
+struct RowGrads {
+    Tensor t;
+    int64_t stride = 0;
+    const float* p() const { return t.defined() ? t.data_ptr<float>() : nullptr; }
 };
 
-// [M, top] or [B, top, N], contiguous
-Top top_of(const OptTensor& t, const Tensor& scores, const Scores& s) {
-    Top r;
-    if (!t.has_value() || !t->defined()) return r;
-    need_cuda(*t, "top");
-    same_device(scores, *t, "top");
-    const bool flat = scores.dim() == 2;
-    TORCH_CHECK(t->dim() == scores.dim() && t->is_contiguous() && t->size(0) == scores.size(0) && (flat || t->size(2) == scores.size(2)),
-                "the top alternatives must be contiguous [M, top] or [B, top, N], got ", t->sizes());
-    TORCH_CHECK(t->size(1) <= 16 && t->size(1) <= s.c, "at most 16 alternatives and the number of classes (", s.c, "), asked for ", t->size(1));
-    r.k = int32_t(t->size(1));
-    if (flat) { r.tk = 1; r.tn = r.k; }
-    else { r.tb = r.k * s.n; r.tk = s.n; r.tn = 1; }
+RowGrads row_grads(const Tensor& t) {
+    RowGrads r;
+    if (!t.defined()) return r;
+    bool expanded = true;
+    for (int64_t d = 0; d < t.dim(); ++d) expanded = expanded && (t.size(d) <= 1 || t.stride(d) == 0);
+    r.t = expanded ? t : t.contiguous();
+    r.stride = expanded ? 0 : 1;
     return r;
 }
 
-const int64_t* top_index_of(const OptTensor& index, const OptTensor& lp) {
-    if (!index.has_value() || !index->defined()) return nullptr;
-    TORCH_CHECK(lp.has_value() && lp->defined() && index->sizes() == lp->sizes() && index->scalar_type() == at::kLong && index->is_contiguous() &&
-                index->device() == lp->device(), "top_index must be contiguous int64 of top_logprob's shape");
-    return index->data_ptr<int64_t>();
+struct Top {
+    int32_t k;
+    int64_t tb, tk, tn;
+};
+
+// layout of the alternatives, contiguous [M, top] or [B, top, N]
+Top top_of(const Tensor& scores, const Scores& s, int64_t top) {
+    TORCH_CHECK(top >= 0 && top <= 16 && top <= s.c, "top must be between 0 and ", s.c < 16 ? s.c : 16, ", got ", top);
+    if (scores.dim() == 2) return Top{int32_t(top), 0, 1, top};
+    return Top{int32_t(top), top * s.n, s.n, 1};
 }
 
-void class_logprobs(const Tensor& scores, const OptTensor& labels, int64_t ignore, const OptTensor& logprob, Tensor& entropy,
-                    const OptTensor& stat, const OptTensor& top_lp, const OptTensor& top_index) {
-    const c10::DeviceGuard guard(scores.device());
-    Scores s = scores_of(scores, "scores");
-    const int64_t rows = s.b * s.n;
-    Top t = top_of(top_lp, scores, s);
-    int64_t* idx = const_cast<int64_t*>(top_index_of(top_index, top_lp));
-    TORCH_CHECK(t.k == 0 || (top_index.has_value() && top_index->defined()), "top_logprob without top_index");
-    if (top_lp.has_value() && top_lp->defined()) TORCH_CHECK(top_lp->scalar_type() == at::kFloat, "top_logprob must be float32");
-    check_rc(mh_class_logprobs(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, labels_of(labels, scores, rows), ignore,
-                               rows_of(logprob, "logprob", scores, rows), rows_of(entropy, "entropy", scores, rows),
-                               rows_of(stat, "stat", scores, 2 * rows), t.k, t.k ? top_lp->data_ptr<float>() : nullptr, idx, t.tb, t.tk, t.tn,
-                               stream_of(scores)), "class_logprobs");
+std::vector<int64_t> rows_shape(const Tensor& scores) {
+    if (scores.dim() == 2) return {scores.size(0)};
+    return {scores.size(0), scores.size(2)};
 }
 
-void class_logprobs_bwd(const Tensor& scores, const OptTensor& labels, int64_t ignore, const Tensor& stat, const Tensor& entropy,
-                        const OptTensor& g_logprob, const OptTensor& g_entropy, const OptTensor& g_top, const OptTensor& top_index,
-                        Tensor& d_scores) {
-    const c10::DeviceGuard guard(scores.device());
-    Scores s = scores_of(scores, "scores"), d = scores_of(d_scores, "d_scores");
-    TORCH_CHECK(d_scores.sizes() == scores.sizes() && d.dtype == s.dtype && d_scores.device() == scores.device(), "d_scores must be like scores");
-    const int64_t rows = s.b * s.n;
-    Top t = top_of(g_top, scores, s);
-    if (t.k) TORCH_CHECK(g_top->scalar_type() == at::kFloat && top_index.has_value(), "g_top must be float32 and come with top_index");
-    auto gl = row_grad(g_logprob, "g_logprob", scores, rows), gh = row_grad(g_entropy, "g_entropy", scores, rows);
-    check_rc(mh_class_logprobs_bwd(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, labels_of(labels, scores, rows), ignore,
-                                   rows_of(stat, "stat", scores, 2 * rows), rows_of(entropy, "entropy", scores, rows), gl.first, gl.second,
-                                   gh.first, gh.second, t.k, t.k ? g_top->data_ptr<float>() : nullptr, t.k ? top_index_of(top_index, g_top) : nullptr,
-                                   t.tb, t.tk, t.tn, d_scores.data_ptr(), d.sb, d.sc, d.sn, stream_of(scores)), "class_logprobs_bwd");
+// labels are read as they are: int64, contiguous, one for each row
+OptTensor check_labels(const OptTensor& labels, const Tensor& scores) {
+    if (!labels.has_value() || !labels->defined()) return OptTensor();
+    TORCH_CHECK(labels->sizes() == at::IntArrayRef(rows_shape(scores)), "labels have shape ", labels->sizes(), ", expected ",
+                at::IntArrayRef(rows_shape(scores)));
+    need_cuda(*labels, "labels");
+    same_device(scores, *labels, "labels");
+    TORCH_CHECK(labels->scalar_type() == at::kLong, "labels must be int64, got ", labels->scalar_type());
+    return labels->contiguous();
 }
 
-void class_nll(const Tensor& scores, const Tensor& labels, int64_t ignore, const OptTensor& stat, Tensor& loss, Tensor& accuracy,
-               Tensor& inv_count) {
-    const c10::DeviceGuard guard(scores.device());
-    Scores s = scores_of(scores, "scores");
-    const int64_t rows = s.b * s.n;
-    const size_t bytes = mh_class_nll_workspace_bytes();
-    Tensor ws = at::empty({int64_t(bytes / sizeof(double))}, scores.options().dtype(at::kDouble));
-    check_rc(mh_class_nll(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, labels_of(labels, scores, rows), ignore,
-                          rows_of(stat, "stat", scores, 2 * rows), rows_of(loss, "loss", scores, 1),
-                          rows_of(accuracy, "accuracy", scores, 1), rows_of(inv_count, "inv_count", scores, 1), ws.data_ptr(), bytes, stream_of(scores)),
-             "class_nll");
+const int64_t* label_ptr(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr<int64_t>() : nullptr; }
+
+// memory for a gradient, in the scores' own layout where that is dense: written as the scores are read
+Tensor grad_like(const Tensor& scores) { return at::empty_like(scores, scores.options().requires_grad(false)); }
+
+struct ClassLogprobs : public torch::autograd::Function<ClassLogprobs> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& scores, const OptTensor& given, int64_t ignore, int64_t top, bool keep) {
+        const c10::DeviceGuard guard(scores.device());
+        const Tensor labels = given.value_or(Tensor());
+        Scores s = scores_of(scores, "scores");
+        const Top t = top_of(scores, s, top);
+        std::vector<int64_t> shape = rows_shape(scores);
+        auto f32 = scores.options().dtype(at::kFloat);
+        Tensor logprob, entropy = at::empty(shape, f32), stat;
+        if (labels.defined()) logprob = at::empty(shape, f32);
+        if (keep) stat = at::empty({s.b * s.n, 2}, f32);
+        shape.insert(shape.begin() + 1, top);
+        Tensor top_lp = at::empty(shape, f32), top_index = at::empty(shape, f32.dtype(at::kLong));
+        check_rc(mh_class_logprobs(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, label_ptr(labels), ignore,
+                                   logprob.defined() ? logprob.data_ptr<float>() : nullptr, entropy.data_ptr<float>(),
+                                   keep ? stat.data_ptr<float>() : nullptr, t.k, top_lp.data_ptr<float>(), top_index.data_ptr<int64_t>(),
+                                   t.tb, t.tk, t.tn, stream_of(scores)), "class_logprobs");
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({top_index});
+        ctx->save_for_backward({scores, labels, stat, entropy, top_index});
+        ctx->saved_data["ignore"] = ignore;
+        if (!labels.defined()) return {entropy, top_lp, top_index};
+        return {entropy, top_lp, top_index, logprob};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list v = ctx->get_saved_variables();
+        const Tensor &scores = v[0], &labels = v[1], &stat = v[2], &entropy = v[3], &top_index = v[4];
+        const Tensor g_lp = grads.size() > 3 ? grads[3] : Tensor();
+        if (!g_lp.defined() && !grads[0].defined() && !grads[1].defined()) return variable_list(5);
+        const c10::DeviceGuard guard(scores.device());
+        Scores s = scores_of(scores, "scores");
+        const RowGrads gl = row_grads(g_lp), gh = row_grads(grads[0]);
+        const bool with_top = grads[1].defined() && top_index.size(1) > 0;
+        const Tensor gt = with_top ? grads[1].contiguous() : Tensor();
+        const Top t = top_of(scores, s, top_index.size(1));
+        Tensor d = grad_like(scores);
+        Scores ds = scores_of(d, "gradient");
+        check_rc(mh_class_logprobs_bwd(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, label_ptr(labels), ctx->saved_data["ignore"].toInt(),
+                                       stat.data_ptr<float>(), entropy.data_ptr<float>(), gl.p(), gl.stride, gh.p(), gh.stride,
+                                       with_top ? t.k : 0, with_top ? gt.data_ptr<float>() : nullptr,
+                                       with_top ? top_index.data_ptr<int64_t>() : nullptr, t.tb, t.tk, t.tn, d.data_ptr(), ds.sb, ds.sc, ds.sn,
+                                       stream_of(scores)), "class_logprobs_bwd");
+        variable_list out = once({d}, "class_logprobs");
+        out.resize(5);
+        return out;
+    }
+};
+
+// (logprob or undefined, entropy, top_logprob, top_index)
+std::tuple<Tensor, Tensor, Tensor, Tensor> class_logprobs(const Tensor& scores, const OptTensor& labels, int64_t ignore, int64_t top) {
+    scores_of(scores, "scores");
+    const bool keep = at::GradMode::is_enabled() && scores.requires_grad();
+    variable_list r = ClassLogprobs::apply(scores, check_labels(labels, scores), ignore, top, keep);
+    return std::make_tuple(r.size() > 3 ? r[3] : Tensor(), r[0], r[1], r[2]);
 }
 
-void class_nll_bwd(const Tensor& scores, const Tensor& labels, int64_t ignore, const Tensor& stat, const Tensor& inv_count, const Tensor& g_loss,
-                   Tensor& d_scores) {
-    const c10::DeviceGuard guard(scores.device());
-    Scores s = scores_of(scores, "scores"), d = scores_of(d_scores, "d_scores");
-    TORCH_CHECK(d_scores.sizes() == scores.sizes() && d.dtype == s.dtype && d_scores.device() == scores.device(), "d_scores must be like scores");
-    const int64_t rows = s.b * s.n;
-    check_rc(mh_class_nll_bwd(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, labels_of(labels, scores, rows), ignore,
-                              rows_of(stat, "stat", scores, 2 * rows), rows_of(inv_count, "inv_count", scores, 1), rows_of(g_loss, "g_loss", scores, 1),
-                              d_scores.data_ptr(), d.sb, d.sc, d.sn, stream_of(scores)), "class_nll_bwd");
+struct ClassNll : public torch::autograd::Function<ClassNll> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& scores, const Tensor& labels, int64_t ignore, bool keep) {
+        const c10::DeviceGuard guard(scores.device());
+        Scores s = scores_of(scores, "scores");
+        auto f32 = scores.options().dtype(at::kFloat);
+        Tensor loss = at::empty({}, f32), accuracy = at::empty({}, f32), inv_count = at::empty({}, f32), stat;
+        if (keep) stat = at::empty({s.b * s.n, 2}, f32);
+        const size_t bytes = mh_class_nll_workspace_bytes();
+        Tensor ws = at::empty({int64_t(bytes / sizeof(double))}, f32.dtype(at::kDouble));
+        check_rc(mh_class_nll(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, label_ptr(labels), ignore, keep ? stat.data_ptr<float>() : nullptr,
+                              loss.data_ptr<float>(), accuracy.data_ptr<float>(), inv_count.data_ptr<float>(), ws.data_ptr(), bytes,
+                              stream_of(scores)), "class_nll");
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({accuracy});
+        ctx->save_for_backward({scores, labels, stat, inv_count});
+        ctx->saved_data["ignore"] = ignore;
+        return {loss, accuracy};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        if (!grads[0].defined()) return variable_list(4);
+        variable_list v = ctx->get_saved_variables();
+        const Tensor& scores = v[0];
+        const c10::DeviceGuard guard(scores.device());
+        Scores s = scores_of(scores, "scores");
+        Tensor d = grad_like(scores);
+        Scores ds = scores_of(d, "gradient");
+        check_rc(mh_class_nll_bwd(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, label_ptr(v[1]), ctx->saved_data["ignore"].toInt(),
+                                  v[2].data_ptr<float>(), v[3].data_ptr<float>(), grads[0].data_ptr<float>(), d.data_ptr(), ds.sb, ds.sc, ds.sn,
+                                  stream_of(scores)), "class_nll_bwd");
+        variable_list out = once({d}, "class_nll");
+        out.resize(4);
+        return out;
+    }
+};
+
+// (mean NLL, accuracy)
+std::tuple<Tensor, Tensor> class_nll(const Tensor& scores, const Tensor& labels, int64_t ignore) {
+    scores_of(scores, "scores");
+    const Tensor lab = check_labels(labels, scores).value_or(Tensor());
+    TORCH_CHECK(lab.defined(), "class_nll needs labels");
+    const bool keep = at::GradMode::is_enabled() && scores.requires_grad();
+    variable_list r = ClassNll::apply(scores, lab, ignore, keep);
+    return std::make_tuple(r[0], r[1]);
 }
 
 // launch width of the calling thread's following cspmm calls (0 = default)
@@ -805,17 +905,10 @@ TORCH_LIBRARY(magnet, m) {
     m.def("ckpt_store(Tensor X, Tensor(a!) codes, Tensor(b!) scales) -> ()");
     m.def("ckpt_restore(Tensor codes, Tensor scales, Tensor(a!) out) -> ()");
     m.def("ckpt_gram(Tensor codes, Tensor scales, int m, Tensor G) -> Tensor");
-    m.def("group_norm(Tensor X, int groups, Tensor? graph_ptr, float eps, Tensor? gamma, Tensor? beta, bool relu, Tensor(a!) out, "
-          "Tensor(b!)? mask, Tensor(c!)? codes, Tensor(d!)? scales) -> Tensor");
-    m.def("group_norm_bwd(Tensor? X, Tensor? codes, Tensor? scales, Tensor? mask, Tensor G, int groups, Tensor? graph_ptr, "
-          "Tensor stats, Tensor? gamma, Tensor? beta, bool relu, Tensor(a!)? dX, Tensor(b!)? dgamma, Tensor(c!)? dbeta) -> ()");
-    m.def("class_logprobs(Tensor scores, Tensor? labels, int ignore, Tensor(a!)? logprob, Tensor(b!) entropy, Tensor(c!)? stat, "
-          "Tensor(d!)? top_logprob, Tensor(e!)? top_index) -> ()");
-    m.def("class_logprobs_bwd(Tensor scores, Tensor? labels, int ignore, Tensor stat, Tensor entropy, Tensor? g_logprob, "
-          "Tensor? g_entropy, Tensor? g_top, Tensor? top_index, Tensor(a!) d_scores) -> ()");
-    m.def("class_nll(Tensor scores, Tensor labels, int ignore, Tensor(a!)? stat, Tensor(b!) loss, Tensor(c!) accuracy, "
-          "Tensor(d!) inv_count) -> ()");
-    m.def("class_nll_bwd(Tensor scores, Tensor labels, int ignore, Tensor stat, Tensor inv_count, Tensor g_loss, Tensor(a!) d_scores) -> ()");
+    m.def("group_norm(Tensor x, Tensor? weight, Tensor? bias, int groups, Tensor? graph_ptr, float eps, bool relu, int bits, "
+          "int next_terms) -> Tensor", &group_norm);
+    m.def("class_logprobs(Tensor scores, Tensor? labels, int ignore, int top) -> (Tensor, Tensor, Tensor, Tensor)", &class_logprobs);
+    m.def("class_nll(Tensor scores, Tensor labels, int ignore) -> (Tensor, Tensor)", &class_nll);
     m.def("set_spmm_grid_cap(int workgroups) -> ()", &set_spmm_grid_cap);
     m.def("noalloc_init(int device_index) -> ()", &noalloc_init);
     m.def("halo_plan(Tensor col_idx, int n_cols, int c0, int c1, Tensor bounds) -> (Tensor, Tensor, Tensor)");
@@ -850,12 +943,6 @@ TORCH_LIBRARY_IMPL(magnet, CUDA, m) {
     m.impl("ckpt_store", &ckpt_store);
     m.impl("ckpt_restore", &ckpt_restore);
     m.impl("ckpt_gram", &ckpt_gram);
-    m.impl("group_norm", &group_norm);
-    m.impl("group_norm_bwd", &group_norm_bwd);
-    m.impl("class_logprobs", &class_logprobs);
-    m.impl("class_logprobs_bwd", &class_logprobs_bwd);
-    m.impl("class_nll", &class_nll);
-    m.impl("class_nll_bwd", &class_nll_bwd);
     m.impl("halo_plan", &halo_plan);
     m.impl("powerlaw_edges", &powerlaw_edges);
     m.impl("stream_read", &stream_read);

@@ -10,40 +10,9 @@ has no normalisation; it is what lets networks of more than a few convolutions t
 """
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .._lib import ops, MagnetHipError
-from ..checkpoint import Checkpoint8, contiguous_columns
-from .sparse_magnet import _alloc_out, _as_packed, _views
-
-
-class _GroupNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, graph_ptr, eps, relu, keep, next_terms):
-        n, _, f = x.shape
-        xc = contiguous_columns(x)
-        out = _alloc_out(n, f, next_terms, x.device)
-        codes = scales = mask = None
-        if keep == 8:                                  # the checkpoint is made by the pass that reads x anyway
-            codes, scales = Checkpoint8.memory(n, f, x.device)
-            mask = torch.empty((n, f), dtype=torch.uint8, device=x.device) if relu else None
-        stats = ops.group_norm(xc, groups, graph_ptr, eps, weight, bias, relu, out, mask, codes, scales)
-        ctx.groups, ctx.relu = groups, relu
-        ctx.save_for_backward(x if codes is None else None, codes, scales, mask, weight, bias, graph_ptr, stats)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, codes, scales, mask, weight, bias, graph_ptr, stats = ctx.saved_tensors
-        n, _, f = g.shape
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty((n, 2, f), dtype=torch.float32, device=g.device) if need_x else None
-        dw = torch.empty_like(weight) if need_w else None
-        db = torch.empty_like(bias) if need_b else None
-        ops.group_norm_bwd(None if x is None else contiguous_columns(x), codes, scales, mask, contiguous_columns(g), ctx.groups, graph_ptr, stats, weight,
-                           bias, ctx.relu, dx, dw, db)
-        return dx, dw, db, None, None, None, None, None, None
+from .sparse_magnet import _as_packed, _views
 
 
 def complex_group_norm(x, num_groups, weight=None, bias=None, graph_ptr=None, eps=1e-5, relu=False, checkpoint_bits=32,
@@ -57,19 +26,13 @@ def complex_group_norm(x, num_groups, weight=None, bias=None, graph_ptr=None, ep
     checkpoint_bits: 32 keeps x itself for the backward pass; 8 keeps a Checkpoint8 of it, and the gate in a byte: the
         gradients are those of the formula with the restored values in the place of x's and the forward's statistics.
     next_terms: above 1, the result is order 0 of a new side-by-side block of that many orders, for the conv that follows."""
-    if x.dim() != 3 or x.size(1) != 2:
-        raise MagnetHipError('x must be row-planar [N, 2, F], got %s' % (tuple(x.shape),))
-    if checkpoint_bits not in (8, 32):
-        raise MagnetHipError('checkpoint_bits is 8 or 32, got %r' % (checkpoint_bits,))
     if not eps >= 0.0:
         raise MagnetHipError('eps must not be negative, got %r' % (eps,))
     if graph_ptr is not None and graph_ptr.dtype != torch.int32:
         if graph_ptr.dtype != torch.int64:
             raise MagnetHipError('graph_ptr must be an integer tensor, got %s' % graph_ptr.dtype)
         graph_ptr = graph_ptr.to(torch.int32)
-    wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
-    return _GroupNormFn.apply(x, weight, bias, int(num_groups), graph_ptr, float(eps), bool(relu), checkpoint_bits if wanted else 32,
-                             next_terms)
+    return ops.group_norm(x, weight, bias, num_groups, graph_ptr, eps, relu, checkpoint_bits, next_terms)
 
 
 class ComplexGroupNorm(nn.Module):
