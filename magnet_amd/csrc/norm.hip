@@ -35,6 +35,7 @@ constexpr int kStats = 5;                  // re mean (high, low), im mean (high
 // the reads of the next pass (1M x 128: sums 199 -> 170 us forward and 379 -> 340 us backward, 6.0 TB/s; the four passes over
 // 200k x 64 together 183 -> 167 us).  Smaller ones stay, for the convolution that comes next.
 constexpr int64_t kPast = int64_t(64) << 20;
+constexpr int64_t kFewPieces = 64;
 constexpr int kMostParts = 16;             // shares of a graph's pieces
 
 struct NormArgs {
@@ -669,7 +670,12 @@ extern "C" int mh_group_norm_bwd(const float* X, int64_t ld, int64_t im, const u
     take_layout(a, l);
     a.tile_rows = l.sum_rows;
     if (any) run_pass(held ? kBwdSumsHeld : kBwdSums, l, a, stream);
-    if (n_graphs > 0)
+    // one graph of few pieces: the pieces are the shares, and need no joining first (2500 x 16: one launch of four)
+    const int64_t tiles = l.sum_pieces - n_graphs;
+    if (any && n_graphs == 1 && !graph_ptr && tiles <= kFewPieces) {
+        a.sums = a.partial;
+        a.parts = int32_t(tiles);
+    } else if (n_graphs > 0)
         norm_bwd_channels_kernel<<<dim3(unsigned(n_graphs), unsigned((F + 31) / 32), unsigned(l.parts)), l.channel_threads, 0, stream>>>(a);
     norm_bwd_means_kernel<<<unsigned((n_graphs * groups + 3) / 4) + unsigned((F + 15) / 16), kBlock, 0, stream>>>(a);
     if (any && dX) run_pass(held ? kBwdApplyHeld : kBwdApply, l, a, stream);

@@ -193,13 +193,16 @@ __device__ inline void place(const ScoreArgs& a, int64_t row, int64_t& b, int64_
 }
 
 // ONE: a row's classes fit its lanes' registers, and the best are taken from there.  Else a lane keeps a list of its TOPN best.
-template <class T, int P, int TOPN, bool NLL, bool ONE, bool JOIN>
+// UNIT: 16 lanes to a row and classes one behind the other, known when compiled: offsets become part of the load instructions.
+template <class T, int P, int TOPN, bool NLL, bool ONE, bool JOIN, bool UNIT>
 __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int rows_of_wave = 64 >> a.ll, lanes = 1 << a.ll;
-    const int r = a.by_class ? lane & (rows_of_wave - 1) : lane >> a.ll;
-    const int l = a.by_class ? lane >> (6 - a.ll) : lane & (lanes - 1);
-    const Group group{lanes, a.by_class ? rows_of_wave : 1};
+    const int ll = UNIT ? 4 : a.ll, rows_of_wave = 64 >> ll, lanes = 1 << ll;
+    const bool by_class = !UNIT && a.by_class;
+    const int64_t sc = UNIT ? 1 : a.sc;
+    const int r = by_class ? lane & (rows_of_wave - 1) : lane >> ll;
+    const int l = by_class ? lane >> (6 - ll) : lane & (lanes - 1);
+    const Group group{lanes, by_class ? rows_of_wave : 1};
     const int waves = kBlock / 64;
     const int64_t step = int64_t(rows_of_wave) * (JOIN ? 1 : waves) * gridDim.x;
     const int64_t first = (int64_t(blockIdx.x) * (JOIN ? 1 : waves) + (JOIN ? 0 : wave)) * rows_of_wave;
@@ -220,12 +223,9 @@ __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
         float of_label = 0.0f;
         for (int32_t c0 = JOIN ? wave * P * lanes : 0; c0 < a.classes; c0 += P * lanes * (JOIN ? waves : 1)) {
             float v[P];
-            const T* at = x + (c0 + l) * a.sc;
+            const T* at = x + (c0 + l) * sc;
 #pragma unroll
-            for (int j = 0; j < P; ++j) {
-                v[j] = live && c0 + j * lanes + l < a.classes ? to_f(*at) : -INFINITY;
-                at += lanes * a.sc;
-            }
+            for (int j = 0; j < P; ++j) v[j] = live && c0 + j * lanes + l < a.classes ? to_f(at[j * lanes * sc]) : -INFINITY;
             if (ONE) acc.m = group.max(largest(v));
             else acc.raise(fmaxf(acc.m, largest(v)));
             acc.add(v);
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kBlock) score_rows(const ScoreArgs a) {
         const bool counted = writes && a.labels && label != a.ignore;
         if (counted) {
             const bool inside = label >= 0 && label < a.classes;
-            if (inside && !(ONE && P == kPer && lanes == 1)) of_label = to_f(x[label * a.sc]);
+            if (inside && !(ONE && P == kPer && lanes == 1)) of_label = to_f(x[label * sc]);
             lp = inside ? (of_label - acc.m) - log_s : NAN;
         }
         if (writes && a.stat) a.stat[row] = make_float2(acc.m, log_s);
@@ -463,7 +463,7 @@ struct Shape {
 };
 
 // Lanes of a row.  Row-major: as many as hold the row at kPer classes each, past 64 classes at kMore each but 16 at least (60k x 349
-// with 5 alternatives: 80 us on 64 lanes of 8, WIDE us on 16 of 24).  Class-major: one, unless there are too few rows to fill the GPU.
+// with 5 alternatives: 80 us on 64 lanes of 8, 47 us on 16 of 24).  Class-major: one, unless there are too few rows to fill the GPU.
 // A workgroup joins on its rows when even whole wavefronts per row are too few for the GPU and every wave gets classes.
 Shape shape_of(int64_t rows, int32_t classes, int64_t sc, int64_t sn, bool can_join, unsigned most) {
     Shape s;
@@ -482,14 +482,20 @@ Shape shape_of(int64_t rows, int32_t classes, int64_t sc, int64_t sn, bool can_j
 
 template <class T, int TOPN, bool NLL>
 void launch_rows(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
-    if (s.join) score_rows<T, kPer, TOPN, NLL, false, true><<<s.blocks, kBlock, 0, stream>>>(a);
-    else score_rows<T, kPer, TOPN, NLL, false, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    if (s.join) score_rows<T, kPer, TOPN, NLL, false, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    else score_rows<T, kPer, TOPN, NLL, false, false, false><<<s.blocks, kBlock, 0, stream>>>(a);
+}
+
+template <class T, bool NLL>
+void launch_one(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
+    if (s.per == kPer) score_rows<T, kPer, 0, NLL, true, false, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    else if (s.ll == 4 && a.sc == 1) score_rows<T, kMore, 0, NLL, true, false, true><<<s.blocks, kBlock, 0, stream>>>(a);
+    else score_rows<T, kMore, 0, NLL, true, false, false><<<s.blocks, kBlock, 0, stream>>>(a);
 }
 
 template <class T>
 void launch_report(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
-    if (s.one && s.per == kMore) score_rows<T, kMore, 0, false, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
-    else if (s.one) score_rows<T, kPer, 0, false, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    if (s.one) launch_one<T, false>(a, s, stream);
     else if (a.top == 0) launch_rows<T, 0, false>(a, s, stream);
     else if (a.top <= 2) launch_rows<T, 2, false>(a, s, stream);
     else if (a.top <= 8) launch_rows<T, 8, false>(a, s, stream);
@@ -512,8 +518,7 @@ void launch_grads(GradArgs a, hipStream_t stream) {
 
 template <class T>
 void launch_nll(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
-    if (s.one && s.per == kMore) score_rows<T, kMore, 0, true, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
-    else if (s.one) score_rows<T, kPer, 0, true, true, false><<<s.blocks, kBlock, 0, stream>>>(a);
+    if (s.one) launch_one<T, true>(a, s, stream);
     else launch_rows<T, 1, true>(a, s, stream);
 }
 
