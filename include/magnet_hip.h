@@ -297,7 +297,7 @@ int mh_relu_bwd_to(const float* G, int64_t ld, int64_t im, const uint8_t* mask,
  *   mh_ckpt_restore  codes, scales -> X
  *   mh_ckpt_gram     out[m][n] = A^T G, A the restored matrix [R][m], G row-planar float32 with n columns (stride 0 allowed):
  *                    the weight gradient of a convolution whose propagated input is held in 8 bits.  Products and sums are
- *                    float32; the same result every time.  A value of G that is not finite makes its column of out NaN.
+ *                    float32; the same result every time.  m * n <= 2^26.  A value of G that is not finite makes its column of out NaN.
  *                    workspace: mh_ckpt_gram_workspace_bytes, contents irrelevant before and after.
  */
 int mh_ckpt_store(const float* X, int64_t ld, int64_t im, int64_t n_rows, int32_t m, uint8_t* codes, uint8_t* scales,
@@ -317,7 +317,7 @@ int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t n_rows, in
  * n_rows; NULL: one graph of all rows).  Group g holds channels g F/groups .. (g+1) F/groups.  With m = mean z (complex) and
  * v = mean |z - m|^2 over a graph's values of a group,
  *     Y = gamma (X - m) / sqrt(v + eps) + beta on both parts  [relu: both parts times (Re Y >= 0)]
- * gamma, beta: float[F] or NULL (1, 0).  Rows behind the last graph are written as zeros; a graph may be empty.
+ * gamma, beta: float[F] or NULL (1, 0).  At most 2^31 rows, 2^22 graphs and 2^25 groups in all.  Rows behind the last graph are written as zeros; a graph may be empty.
  * stats: float[n_graphs * groups * MH_NORM_STATS], for the backward pass.  mask_out: uint8 [n_rows][F] or NULL, the gate.
  * codes_out, scales_out: a checkpoint of X as mh_ckpt_store makes it, or both NULL.
  *   mh_group_norm_bwd  dX, dgamma, dbeta (each may be NULL) from the gradient G of Y.  The input is X, or, where codes is not

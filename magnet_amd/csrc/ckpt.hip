@@ -468,7 +468,7 @@ extern "C" int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t
                             int64_t img, int32_t n, float* out, void* workspace, size_t workspace_bytes, void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     if (int rc = check_checkpoint(codes, scales, n_rows, m)) return rc;
-    MH_REQUIRE(n >= 1 && int64_t(m) * n <= (int64_t(1) << 30), "m=%d n=%d", m, n);
+    MH_REQUIRE(n >= 1 && int64_t(m) * n <= (int64_t(1) << 26), "m=%d n=%d", m, n);
     MH_REQUIRE(out, "null pointer");
     MH_REQUIRE(ldg >= 0 && img >= 0 && ldg <= (1 << 24) && img <= (int64_t(1) << 40), "row stride of G: %lld", (long long)ldg);
     GramArgs a{};

@@ -89,7 +89,9 @@ __device__ inline Piece piece_of(const NormArgs& a, int64_t d) {
     if (a.ptr) {
         for (int32_t n = a.graphs + 1; n > 1;) {
             const int32_t step = (n + 63) >> 6, at = int32_t(threadIdx.x & 63) * step;
-            const int32_t below = __popcll(__ballot(at < n && first_piece(a, lo + at) <= d)) - 1;
+            // the candidates up to the first that begins behind d; the first of all does not, whatever ptr holds
+            const uint64_t behind = ~__ballot(at < n && first_piece(a, lo + at) <= d);
+            const int32_t first = behind ? __ffsll(static_cast<unsigned long long>(behind)) - 1 : 64, below = first > 0 ? first - 1 : 0;
             const int32_t left = n - below * step;
             lo += below * step;
             n = left < step ? left : step;
@@ -554,7 +556,7 @@ Workspace workspace_of(int64_t rows, int32_t graphs, int32_t F, int32_t groups) 
 int check_norm(int64_t rows, int32_t F, int32_t groups, const void* ptr, int32_t graphs) {
     MH_REQUIRE(rows >= 0 && rows <= INT32_MAX && F >= 1 && F <= (1 << 20), "n_rows=%lld F=%d", (long long)rows, F);
     MH_REQUIRE(groups >= 1 && F % groups == 0, "%d channels do not divide into %d groups", F, groups);
-    MH_REQUIRE(graphs >= (rows > 0 ? 1 : 0) && graphs <= (1 << 24) && int64_t(graphs) * groups <= (int64_t(1) << 30), "n_graphs=%d", graphs);
+    MH_REQUIRE(graphs >= (rows > 0 ? 1 : 0) && graphs <= (1 << 22) && int64_t(graphs) * groups <= (int64_t(1) << 25), "n_graphs=%d", graphs);
     MH_REQUIRE(ptr || graphs <= 1, "n_graphs=%d without graph_ptr", graphs);
     return MH_OK;
 }

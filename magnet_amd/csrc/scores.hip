@@ -507,7 +507,7 @@ void launch_grads(GradArgs a, hipStream_t stream) {
     constexpr int E = 16 / sizeof(T);
     const int64_t total = a.rows * a.classes, blocks = (total + int64_t(kBlock) * E - 1) / (int64_t(kBlock) * E);
     const bool dense = a.rows == a.inner && a.sc == 1 && a.dc == 1 && a.sn == a.classes && a.dn == a.classes && a.classes >= E;
-    if (dense && blocks <= INT32_MAX && mh_aligned16(a.x) && mh_aligned16(a.d)) {
+    if (dense && blocks <= (1 << 23) && mh_aligned16(a.x) && mh_aligned16(a.d)) {
         score_grads_flat<T, NLL><<<unsigned(blocks), kBlock, 0, stream>>>(a);
         return;
     }

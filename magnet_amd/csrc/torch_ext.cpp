@@ -453,7 +453,7 @@ Batch batch_of(const OptTensor& graph_ptr, const Tensor& x, int64_t n) {
     if (!graph_ptr.has_value() || !graph_ptr->defined()) { b.n = n ? 1 : 0; return b; }
     b.ptr = i32(*graph_ptr, "graph_ptr");
     same_device(x, *graph_ptr, "graph_ptr");
-    TORCH_CHECK(graph_ptr->dim() == 1 && graph_ptr->numel() >= 1 && graph_ptr->numel() <= (1 << 24), "graph_ptr must hold n_graphs + 1 row numbers");
+    TORCH_CHECK(graph_ptr->dim() == 1 && graph_ptr->numel() >= 1 && graph_ptr->numel() <= (1 << 22), "graph_ptr must hold n_graphs + 1 row numbers");
     b.n = int32_t(graph_ptr->numel() - 1);
     return b;
 }
@@ -528,6 +528,8 @@ using torch::autograd::variable_list;
 // gradients that are not differentiable themselves: asked to be (create_graph), they raise when it comes to that
 variable_list once(variable_list grads, const char* what) {
     if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor& g : grads)
+        if (g.defined()) g = g.detach().set_requires_grad(true);
     auto error = std::make_shared<torch::autograd::DelayedError>(std::string("the gradient of ") + what + " cannot be differentiated again",
                                                                  int64_t(grads.size()));
     return (*error)(std::move(grads));

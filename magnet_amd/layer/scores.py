@@ -16,6 +16,7 @@ from collections import namedtuple
 from .._lib import ops
 
 IGNORE = -100                  # torch's default ignore_index
+MOST_TOP = 16                  # alternatives of a row
 
 ClassLogprobs = namedtuple('ClassLogprobs', 'logprob entropy top_logprob top_index')
 

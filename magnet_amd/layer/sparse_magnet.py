@@ -346,7 +346,6 @@ class _ChebConvFn(torch.autograd.Function):
             if need_w:                                     # X^T [T_0 G ... T_K G] -> [C_in, K+1, C_out]
                 xg = _gram(_rows2(xp), _block_rows(ds)) if ctx.held is None else ctx.held.gram(ds)
                 dw = xg.view(cin, k1, cout).permute(1, 0, 2).contiguous()
-            ctx.held = None
             if need_x:
                 dx = torch.mm(_block_rows(ds), w.transpose(1, 2).reshape(k1 * cout, cin)).view(n, 2, cin)
         else:
@@ -357,6 +356,8 @@ class _ChebConvFn(torch.autograd.Function):
             if need_w and ctx.held is not None:
                 dw = ctx.held.gram(g).view(k1, cin, cout)
             elif need_w:
+                if ctx.block is None and ctx.x0 is None:
+                    raise MagnetHipError('the saved orders were let go by an earlier backward pass of this graph')
                 block = ctx.block if ctx.block is not None else _cheb_terms(lap, ctx.x0, k1)   # recomputed orders
                 dw = _gram(_block_rows(block), g2).view(k1, cin, cout)
                 block = None

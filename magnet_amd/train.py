@@ -12,7 +12,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
-from .layer.scores import IGNORE, class_logprobs, class_nll          # IGNORE: F.nll_loss's default ignore_index
+from .layer.scores import IGNORE, MOST_TOP, class_logprobs, class_nll          # IGNORE: F.nll_loss's default ignore_index
 
 
 class NodeTargets:
@@ -313,10 +313,10 @@ class GraphedEpoch:
 def save_report(path, model, labels, top, X_real, X_img, *index):
     """Writes `path`.npz: the log probability of every row's label, the entropy of its distribution and its `top` best classes
     with their log probabilities, under the model's current weights.  `labels` as the network answers: [1, N], or [M] with the
-    node pairs as `index`.  `top` is cut to the number of classes."""
+    node pairs as `index`.  `top` is cut to the number of classes and to 16."""
     model.eval()
     with torch.no_grad():
         scores = _answer(model, True, X_real, X_img, *index)
-        r = class_logprobs(scores, labels, top=min(top, scores.size(1)))
+        r = class_logprobs(scores, labels, top=min(top, scores.size(1), MOST_TOP))
     np.savez(path, logprob=r.logprob.cpu().numpy(), entropy=r.entropy.cpu().numpy(), top_logprob=r.top_logprob.cpu().numpy(),
              top_index=r.top_index.cpu().numpy())

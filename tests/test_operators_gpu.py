@@ -871,3 +871,147 @@ def test_drivers_take_the_new_arguments(tmp_path):
         assert set(r.files) == {'logprob', 'entropy', 'top_logprob', 'top_index'}
         assert (r['entropy'] >= -1e-6).all() and np.isfinite(r['logprob']).all() and r['top_index'].shape[1] == 2
         assert (np.diff(r['top_logprob'], axis=1) <= 0).all()
+
+
+# ---------------------------------------------------------------------------------------------
+# the C ABI with raw pointers, and calls at the edges of what the documentation allows
+# ---------------------------------------------------------------------------------------------
+def test_entry_points_with_raw_pointers():
+    """Every entry point of the three operators as a caller without torch binds it, against the operators of the extension."""
+    from magnet_amd import _lib
+    from magnet_amd._lib import lib, ptr, stream_ptr, check
+    from magnet_amd.checkpoint import Checkpoint8
+    from magnet_amd.layer.norm import complex_group_norm
+    from magnet_amd.layer.scores import class_logprobs, class_nll
+    n, f, k, s = 301, 20, 6, stream_ptr(torch.device(DEV, 0))
+    x, g = _features(n, f, seed=1).to(DEV), torch.randn(n, 2, k, generator=_gen(2)).to(DEV)
+    empty = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=DEV)
+    ck = Checkpoint8.store(x)
+    codes, scales, back, dw = torch.empty_like(ck.codes), torch.empty_like(ck.scales), torch.empty_like(x), empty(f, k)
+    check(lib.mh_ckpt_store(ptr(x), 2 * f, f, n, f, ptr(codes), ptr(scales), s))
+    check(lib.mh_ckpt_restore(ptr(codes), ptr(scales), n, f, ptr(back), 2 * f, f, s))
+    size = lib.mh_ckpt_gram_workspace_bytes(n, f, k)
+    ws = empty(size, dtype=torch.uint8)
+    check(lib.mh_ckpt_gram(ptr(codes), ptr(scales), n, f, ptr(g), 2 * k, k, k, ptr(dw), ptr(ws), size, s))
+    assert torch.equal(codes, ck.codes) and torch.equal(scales, ck.scales) and torch.equal(back, ck.restore()) and torch.equal(dw, ck.gram(g))
+    w, b = (torch.rand(f, generator=_gen(i)).to(DEV) + 0.5 for i in (3, 4))
+    go = torch.randn(n, 2, f, generator=_gen(5)).to(DEV)
+    graphs = torch.tensor([0, 100, 290], dtype=torch.int32, device=DEV)
+    size = lib.mh_group_norm_workspace_bytes(n, 2, f, 4)
+    ws = empty(size, dtype=torch.uint8)
+    for held in (False, True):
+        xr, wr, br = (t.clone().requires_grad_() for t in (x, w, b))
+        want = complex_group_norm(xr, 4, wr, br, graph_ptr=graphs, relu=True, checkpoint_bits=8 if held else 32)
+        want.backward(go)
+        y, mask, stats, dx, dgamma, dbeta = torch.empty_like(x), empty(n, f, dtype=torch.uint8), empty(2, 4, 5), torch.empty_like(x), empty(f), empty(f)
+        check(lib.mh_group_norm(ptr(x), 2 * f, f, n, f, 4, ptr(graphs), 2, 1e-5, ptr(w), ptr(b), 1, ptr(y), 2 * f, f, ptr(mask),
+                                ptr(codes) if held else None, ptr(scales) if held else None, ptr(stats), ptr(ws), size, s))
+        check(lib.mh_group_norm_bwd(None if held else ptr(x), 2 * f, f, ptr(codes) if held else None, ptr(scales) if held else None, ptr(mask),
+                                    n, f, 4, ptr(graphs), 2, ptr(stats), ptr(w), ptr(b), 1, ptr(go), 2 * f, f, ptr(dx), 2 * f, f, ptr(dgamma),
+                                    ptr(dbeta), ptr(ws), size, s))
+        assert torch.equal(y, want) and torch.equal(dx, xr.grad) and torch.equal(dgamma, wr.grad) and torch.equal(dbeta, br.grad)
+        check(lib.mh_group_norm_bwd(None if held else ptr(x), 2 * f, f, ptr(codes) if held else None, ptr(scales) if held else None, ptr(mask),
+                                    n, f, 4, ptr(graphs), 2, ptr(stats), ptr(w), ptr(b), 1, ptr(go), 2 * f, f, None, 0, 0, ptr(dgamma), None,
+                                    ptr(ws), size, s))               # some gradients not wanted
+        assert torch.equal(dgamma, wr.grad)
+    c = 7
+    sc = torch.randn(n, c, generator=_gen(6)).to(DEV).requires_grad_()
+    lab = torch.randint(0, c, (n,), generator=_gen(7)).to(DEV)
+    r = class_logprobs(sc, lab, top=3)
+    gl, gh, gt = torch.randn(n, device=DEV), torch.randn(n, device=DEV), torch.randn(n, 3, device=DEV)
+    torch.autograd.backward([r.logprob, r.entropy, r.top_logprob], [gl, gh, gt])
+    lp, ent, stat, tl, ti, d = empty(n), empty(n), empty(n, 2), empty(n, 3), empty(n, 3, dtype=torch.int64), empty(n, c)
+    check(lib.mh_class_logprobs(ptr(sc), 0, 1, n, c, 0, 1, c, ptr(lab), -100, ptr(lp), ptr(ent), ptr(stat), 3, ptr(tl), ptr(ti), 0, 1, 3, s))
+    check(lib.mh_class_logprobs_bwd(ptr(sc), 0, 1, n, c, 0, 1, c, ptr(lab), -100, ptr(stat), ptr(ent), ptr(gl), 1, ptr(gh), 1, 3, ptr(gt), ptr(ti),
+                                    0, 1, 3, ptr(d), 0, 1, c, s))
+    assert torch.equal(lp, r.logprob) and torch.equal(ent, r.entropy) and torch.equal(tl, r.top_logprob) and torch.equal(ti, r.top_index)
+    assert torch.equal(d, sc.grad)
+    sc.grad = None
+    loss, acc = class_nll(sc, lab)
+    loss.backward()
+    out, one = empty(3), torch.ones((), device=DEV)
+    size = lib.mh_class_nll_workspace_bytes()
+    ws = empty(size, dtype=torch.uint8)
+    at = lambda t, i: ptr(t[i:])
+    check(lib.mh_class_nll(ptr(sc), 0, 1, n, c, 0, 1, c, ptr(lab), -100, ptr(stat), at(out, 0), at(out, 1), at(out, 2), ptr(ws), size, s))
+    check(lib.mh_class_nll_bwd(ptr(sc), 0, 1, n, c, 0, 1, c, ptr(lab), -100, ptr(stat), at(out, 2), ptr(one), ptr(d), 0, 1, c, s))
+    assert float(out[0]) == float(loss.detach()) and float(out[1]) == float(acc) and torch.equal(d, sc.grad)
+
+
+def test_group_norm_stays_in_bounds_for_graph_borders_that_do_not_ascend():
+    """graph_ptr lies on the GPU and is not read on the host: borders that break its rule give rows of no defined value, and the
+    kernels clamp what they read from it."""
+    from magnet_amd.layer.norm import complex_group_norm
+    n, f = 500, 8
+    x = _features(n, f, seed=1).to(DEV)
+    many = torch.randint(-1000, 2000, (3000,), generator=_gen(2)).to(torch.int32)
+    for p in ([0, 400, 100, 500], [700, 3, -5, 2 ** 31 - 1], [5, 5, 5], many.tolist()):
+        complex_group_norm(x, 2, graph_ptr=torch.tensor(p, device=DEV, dtype=torch.int32), relu=True)
+        xr = x.clone().requires_grad_()
+        complex_group_norm(xr, 2, graph_ptr=torch.tensor(p, device=DEV, dtype=torch.int32), checkpoint_bits=8).backward(x)
+        torch.cuda.synchronize()
+    want = complex_group_norm(x, 2)
+    assert torch.equal(complex_group_norm(x, 2, graph_ptr=torch.tensor([0, n], device=DEV)), want)
+
+
+def test_backward_of_a_kept_graph():
+    """retain_graph: the norm, the scores and the GEMM-first convolution answer again; a convolution that let its orders go says so."""
+    from magnet_amd import MagnetHipError
+    from magnet_amd.layer.norm import complex_group_norm
+    from magnet_amd.layer.scores import class_nll
+    from magnet_amd.layer.sparse_magnet import ChebConv
+    from magnet_amd.utils.hermitian import ChebBasis
+    x = _features(50, 8, seed=1).to(DEV).requires_grad_()
+    y = complex_group_norm(x, 2, relu=True, checkpoint_bits=8)
+    s = torch.randn(9, 4, device=DEV, requires_grad=True)
+    loss, _ = class_nll(s, torch.zeros(9, dtype=torch.int64, device=DEV))
+    for out, leaf in ((y.sum() + (y * y).sum(), x), (loss, s)):
+        out.backward(retain_graph=True)
+        first = leaf.grad.clone()
+        leaf.grad = None
+        out.backward()
+        assert torch.equal(first, leaf.grad)
+    with pytest.raises(RuntimeError, match='differentiated again'):
+        g, = torch.autograd.grad(class_nll(s, torch.zeros(9, dtype=torch.int64, device=DEV))[0], s, create_graph=True)
+        g.sum().backward()
+    lap = _graph(60, 300)
+    for cin, cout in ((8, 4), (4, 8)):
+        conv = ChebConv(cin, cout, 2, ChebBasis(lap, 2), None).to(DEV)
+        conv.checkpoint_bits = 8
+        out = conv.forward_packed(_features(60, cin, seed=2).to(DEV)).sum()
+        out.backward(retain_graph=True)
+        first = conv.weight.grad.clone()
+        conv.weight.grad = None
+        if cout < cin:
+            out.backward()
+            assert torch.equal(first, conv.weight.grad)
+        else:
+            with pytest.raises(MagnetHipError, match='earlier backward'):
+                out.backward()
+
+
+def test_operators_share_a_gpu_between_streams_and_threads():
+    """The same calls from two streams at once, each with workspaces of its own: the results of one after the other."""
+    from magnet_amd.checkpoint import Checkpoint8
+    from magnet_amd.layer.norm import complex_group_norm
+    from magnet_amd.layer.scores import class_nll
+    n = 20000
+    xs = [_features(n, 32, seed=k).to(DEV) for k in (1, 2)]
+    ss = [torch.randn(1, 5, n, generator=_gen(k)).to(DEV) for k in (3, 4)]
+    lab = torch.randint(0, 5, (1, n), generator=_gen(5)).to(DEV)
+
+    def body(x, s):
+        return [complex_group_norm(x, 4, relu=True), Checkpoint8.store(x).gram(x), *class_nll(s, lab)]
+
+    want = [body(x, s) for x, s in zip(xs, ss)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(body(xs[i], ss[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
