@@ -348,47 +348,52 @@ struct GradArgs {
     int64_t tb, tk, tn;
 };
 
-// d x_c = [c = y] g_y + sum_t [c = i_t] g_t - p_c (g_y + sum_t g_t) - p_c (log p_c + H) g_H: what it takes of a row
+// d x_c = [c = y] g_y + sum_t [c = i_t] g_t - p_c (a + g_H log p_c) with a = g_y + sum_t g_t + g_H H: what it takes of a row.  log p is
+// kept above kLowest, where p is 0 already, so that a class without probability multiplies no infinity; a row without a
+// distribution has a = NaN, one that no gradient reaches has p = 0 whatever it holds.
+constexpr float kLowest = -200.0f;
 struct RowGrad {
     int64_t at;                             // of the alternatives
     int32_t label;                          // -1: none
-    float gy, gh, h, all, m, log_s;
-    bool any;
+    float gy, gh, a, m, log_s;
 };
 
 template <bool NLL>
 __device__ inline RowGrad row_grad(const GradArgs& a, int64_t row, int64_t b, int64_t i, float scale) {
     RowGrad r;
+    // all of a row's values are asked for before the first is looked at: one wait instead of one for each
     const int64_t label = a.labels ? a.labels[row] : a.ignore;
-    const bool counted = a.labels && label != a.ignore, inside = label >= 0 && label < a.classes;
-    r.label = counted && inside ? int32_t(label) : -1;
-    r.gy = !counted ? 0.0f : !inside ? NAN : NLL ? scale : a.g_lp ? a.g_lp[row * a.g_lp_s] : 0.0f;      // NaN as its log probability
+    const float gl = NLL ? scale : a.g_lp ? a.g_lp[row * a.g_lp_s] : 0.0f;
+    const float entropy = !NLL && a.g_h ? a.entropy[row] : 0.0f;
+    const float2 st = a.stat[row];
     r.gh = !NLL && a.g_h ? a.g_h[row * a.g_h_s] : 0.0f;
-    r.h = !NLL && a.g_h ? a.entropy[row] : 0.0f;
-    r.all = r.gy;
-    r.any = r.gy != 0.0f || r.gh != 0.0f;
+    const bool counted = label != a.ignore, inside = label >= 0 && label < a.classes;
+    r.label = counted && inside ? int32_t(label) : -1;
+    r.gy = !counted ? 0.0f : !inside ? NAN : gl;                     // NaN as its log probability
+    r.a = r.gy;
+    bool any = r.gy != 0.0f || r.gh != 0.0f;
     r.at = b * a.tb + i * a.tn;
     if (!NLL && a.g_top)
         for (int t = 0; t < a.top; ++t) {
             const float g = a.g_top[r.at + t * a.tk];
-            r.all += g;
-            r.any |= g != 0.0f;
+            r.a += g;
+            any |= g != 0.0f;
         }
-    const float2 st = a.stat[row];
+    r.a = fmaf(r.gh, r.gh != 0.0f ? entropy : 0.0f, r.a);
     r.m = st.x;
     r.log_s = st.y;
+    if (!any) { r.a = 0.0f; r.log_s = INFINITY; }
+    else if (st.y != st.y) r.a = NAN;
     return r;
 }
 
 template <bool NLL>
-__device__ inline float score_grad(const GradArgs& a, const RowGrad& r, float x, int32_t c) {
-    if (!r.any) return 0.0f;                // a row no gradient reaches stays clean whatever it holds
-    const float lp = (x - r.m) - r.log_s, p = weight(lp);
-    float g = (c == r.label ? r.gy : 0.0f) - p * r.all;
-    if (!NLL && a.g_h) g -= p == 0.0f ? 0.0f : p * (lp + r.h) * r.gh;
+__device__ inline float score_grad(const GradArgs& a, const RowGrad& r, float x, int32_t c, int32_t shift) {   // class c + shift
+    const float lp = fmaxf((x - r.m) - r.log_s, kLowest), p = weight(lp);
+    float g = (c == r.label ? r.gy : 0.0f) - p * (NLL ? r.a : fmaf(r.gh, lp, r.a));
     if (!NLL && a.g_top)
         for (int t = 0; t < a.top; ++t)
-            if (a.top_idx[r.at + t * a.tk] == c) g += a.g_top[r.at + t * a.tk];
+            if (a.top_idx[r.at + t * a.tk] == c + shift) g += a.g_top[r.at + t * a.tk];
     return g;
 }
 
@@ -416,7 +421,7 @@ __global__ void __launch_bounds__(kBlock) score_grads(const GradArgs a) {
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
                 const int32_t c = c0 + j * lanes;
-                if (c < a.classes) d[c * a.dc] = from_f<T>(score_grad<NLL>(a, g, v[j], c));
+                if (c < a.classes) d[c * a.dc] = from_f<T>(score_grad<NLL>(a, g, v[j], c, 0));
             }
         }
     }
@@ -441,14 +446,17 @@ __global__ void __launch_bounds__(kBlock) score_grads_flat(const GradArgs a) {
     else
         for (int e = 0; e < E; ++e)
             if (first + e < total) in.v[e] = x[e];
-    const RowGrad g0 = row_grad<NLL>(a, row, 0, row, scale);
-    RowGrad g1 = g0;
-    if (c0 + E > a.classes && row + 1 < a.rows) g1 = row_grad<NLL>(a, row + 1, 0, row + 1, scale);
+    const int64_t after = row + 1 < a.rows ? row + 1 : row;
+    RowGrad g = row_grad<NLL>(a, row, 0, row, scale), g1 = row_grad<NLL>(a, after, 0, after, scale);
+    g.label -= c0;                                                  // as an element of this piece
+    g1.label = g1.label < 0 ? -1 : g1.label + a.classes - c0;
+    const int32_t border = a.classes - c0;
     Pack out;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const bool next = c0 + e >= a.classes;
-        out.v[e] = from_f<T>(score_grad<NLL>(a, next ? g1 : g0, to_f(in.v[e]), next ? c0 + e - a.classes : c0 + e));
+        if (e == border) g = g1;
+        float d1 = score_grad<NLL>(a, g, to_f(in.v[e]), e, e < border ? c0 : -border);
+        out.v[e] = from_f<T>(d1);
     }
     if (whole) *reinterpret_cast<Pack*>(d) = out;
     else
