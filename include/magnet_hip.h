@@ -297,7 +297,7 @@ int mh_relu_bwd_to(const float* G, int64_t ld, int64_t im, const uint8_t* mask,
  *   mh_ckpt_restore  codes, scales -> X
  *   mh_ckpt_gram     out[m][n] = A^T G, A the restored matrix [R][m], G row-planar float32 with n columns (stride 0 allowed):
  *                    the weight gradient of a convolution whose propagated input is held in 8 bits.  Products and sums are
- *                    float32; the same result every time.  m * n <= 2^26.  A value of G that is not finite makes its column of out NaN.
+ *                    float32; the same result every time.  m * n <= 2^24.  A value of G that is not finite makes its column of out NaN.
  *                    workspace: mh_ckpt_gram_workspace_bytes, contents irrelevant before and after.
  */
 int mh_ckpt_store(const float* X, int64_t ld, int64_t im, int64_t n_rows, int32_t m, uint8_t* codes, uint8_t* scales,

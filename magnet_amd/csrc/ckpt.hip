@@ -156,7 +156,7 @@ template <class T>
 __device__ inline T at(const void* base, uint32_t offset) { return *reinterpret_cast<const T*>(static_cast<const char*>(base) + offset); }
 
 constexpr int kRows = 32;                  // rows of a step
-constexpr int64_t kLeast = 128;          // rows of a slab: below, the sums to join cost more than the rows
+constexpr int64_t kLeast = 128;            // rows of a slab: below, the sums to join cost more than the rows
 
 template <int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) ckpt_gram_kernel(const GramArgs a) {
@@ -343,14 +343,16 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) ckpt_gram_kernel(const GramAr
                 out[(wr + i * 32 + 8 * (k >> 2) + 4 * (lane >> 5) + (k & 3)) * BN + wc + j * 32 + (lane & 31)] = acc[i][j][k];
 }
 
-// the slabs' partial sums, in order; 64 results to a workgroup, its waves take a share of the slabs each
+// The slabs' partial sums: O results to a workgroup, 1024 / O threads to a result, each with every so many-th slab, joined in a
+// fixed order.  16 where the result is small, for more workgroups (940 slabs of 120 x 30: 8.7 us, with 64 results 10.4), else 64,
+// for whole lines (256 slabs of 384 x 128: 11 us, with 16 results 21).
 constexpr int kJoin = 1024;
+template <int O>
 __global__ void __launch_bounds__(kJoin) ckpt_gram_join(const float* __restrict__ partial, int32_t slabs, int32_t tiles_m, int32_t tiles_n,
-                                                         int32_t bm, int32_t bn, int32_t m, int32_t n, float* __restrict__ out) {
-    constexpr int waves = kJoin / 64;
-    __shared__ double part[waves][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int32_t e = int32_t(blockIdx.x) * 64 + lane;
+                                                        int32_t bm, int32_t bn, int32_t m, int32_t n, float* __restrict__ out) {
+    __shared__ double part[kJoin / 64][O];
+    const int o = threadIdx.x % O, q = threadIdx.x / O, wave = threadIdx.x >> 6;
+    const int32_t e = int32_t(blockIdx.x) * O + o;
     const bool in = e < m * n;
     double sum = 0.0;
     if (in) {
@@ -358,14 +360,15 @@ __global__ void __launch_bounds__(kJoin) ckpt_gram_join(const float* __restrict_
         const int32_t tile = i / bm + (j / bn) * tiles_m, ii = i % bm;
         const float* p = partial + int64_t(tile) * bm * bn + ((ii & 3) * (bm / 4) + (ii >> 2)) * bn + j % bn;
         const int64_t step = int64_t(tiles_m) * tiles_n * bm * bn;
-        const int32_t s0 = slabs * wave / waves, s1 = slabs * (wave + 1) / waves;
 #pragma unroll 8
-        for (int32_t s = s0; s < s1; ++s) sum += double(p[s * step]);
+        for (int32_t s = q; s < slabs; s += kJoin / O) sum += double(p[s * step]);
     }
-    part[wave][lane] = sum;
+#pragma unroll
+    for (int k = O; k < 64; k <<= 1) sum += __shfl_xor(sum, k);
+    if ((threadIdx.x & 63) < O) part[wave][o] = sum;
     __syncthreads();
-    if (wave == 0 && in) {
-        for (int w = 1; w < waves; ++w) sum += part[w][lane];
+    if (threadIdx.x < O && in) {
+        for (int w = 1; w < kJoin / 64; ++w) sum += part[w][o];
         out[e] = float(sum);
     }
 }
@@ -388,7 +391,9 @@ GramPlan gram_plan(int64_t rows, int32_t m, int32_t n) {
     const int64_t want = (256 * held) / (p.tiles_m * p.tiles_n);
     int64_t each = want > 1 ? (rows + want - 1) / want : rows;
     each = (each + kRows - 1) / kRows * kRows;
-    p.slab_rows = each < kLeast ? kLeast : each;
+    // half of that where there would be few slabs (5000 x 48 x 16: 9.3 us, with 128 rows 10.4, with 256 12.4)
+    const int64_t least = rows < 64 * kLeast ? kLeast / 2 : kLeast;
+    p.slab_rows = each < least ? least : each;
     p.slabs = int32_t((rows + p.slab_rows - 1) / p.slab_rows);
     return p;
 }
@@ -468,7 +473,7 @@ extern "C" int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t
                             int64_t img, int32_t n, float* out, void* workspace, size_t workspace_bytes, void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     if (int rc = check_checkpoint(codes, scales, n_rows, m)) return rc;
-    MH_REQUIRE(n >= 1 && int64_t(m) * n <= (int64_t(1) << 26), "m=%d n=%d", m, n);
+    MH_REQUIRE(n >= 1 && int64_t(m) * n <= (int64_t(1) << 24), "m=%d n=%d", m, n);
     MH_REQUIRE(out, "null pointer");
     MH_REQUIRE(ldg >= 0 && img >= 0 && ldg <= (1 << 24) && img <= (int64_t(1) << 40), "row stride of G: %lld", (long long)ldg);
     GramArgs a{};
@@ -495,7 +500,9 @@ extern "C" int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t
         }
         MH_LAUNCH_CHECK("ckpt_gram");
     }
-    ckpt_gram_join<<<unsigned((int64_t(m) * n + 63) / 64), kJoin, 0, stream>>>(a.partial, a.slabs, a.tiles_m, a.tiles_n, p.bm, p.bn, m, n, out);
+    const int32_t results = m * n;
+    if (results < 64 * 256) ckpt_gram_join<16><<<unsigned(results + 15) / 16, kJoin, 0, stream>>>(a.partial, a.slabs, a.tiles_m, a.tiles_n, p.bm, p.bn, m, n, out);
+    else ckpt_gram_join<64><<<unsigned(results + 63) / 64, kJoin, 0, stream>>>(a.partial, a.slabs, a.tiles_m, a.tiles_n, p.bm, p.bn, m, n, out);
     MH_LAUNCH_CHECK("ckpt_gram_join");
     return MH_OK;
 }
