@@ -9,8 +9,8 @@ cd "${GRAFT_REPO_ROOT:-$(dirname "$0")/..}"
 D=ab/asan
 if [ "${1:-build}" = build ]; then
   mkdir -p $D
-  for f in lap_build radix_sort cspmm aux halo exchange; do
-    /opt/rocm/bin/hipcc -O1 -g -std=c++17 -fPIC --offload-arch=gfx950 -Xarch_host -fsanitize=address -Xarch_host -fno-omit-frame-pointer \
+  for f in lap_build radix_sort cspmm aux halo exchange ckpt norm scores; do
+    /opt/rocm/bin/hipcc -O1 -g -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Xarch_host -fsanitize=address -Xarch_host -fno-omit-frame-pointer \
         -c magnet_amd/csrc/$f.hip -o $D/$f.o || exit 1
   done
   /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -Xarch_host -fsanitize=address $D/*.o -o $D/libmagnet_hip_asan.so -ldl || exit 1

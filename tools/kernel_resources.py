@@ -11,7 +11,8 @@ import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SRC = os.path.join(ROOT, 'magnet_amd', 'csrc')
-FLAGS = ['-O3', '-std=c++17', '-fPIC', '--offload-arch=gfx950', '-Wno-unused-function', '-Rpass-analysis=kernel-resource-usage']
+FLAGS = ['-O3', '-std=c++17', '-fPIC', '--offload-arch=gfx950', '-Wno-unused-function', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
+         '-Rpass-analysis=kernel-resource-usage']
 
 
 def demangle(names):
@@ -28,7 +29,7 @@ def main():
     print('kernel resource usage, gfx950, hipcc %s' % ' '.join(FLAGS[:4]))
     print('occupancy = waves per SIMD the register and LDS budget allows (8 is the hardware maximum; a CU has 4 SIMDs, 160 KiB of LDS)')
     print('%-14s %-58s %6s %6s %6s %8s %9s %10s' % ('file', 'kernel', 'VGPRs', 'AGPRs', 'SGPRs', 'scratch', 'LDS bytes', 'waves/SIMD'))
-    for f in ['cspmm.hip', 'radix_sort.hip', 'lap_build.hip', 'halo.hip', 'aux.hip']:
+    for f in ['cspmm.hip', 'radix_sort.hip', 'lap_build.hip', 'halo.hip', 'aux.hip', 'ckpt.hip', 'norm.hip', 'scores.hip']:
         r = subprocess.run(['/opt/rocm/bin/hipcc'] + FLAGS + ['-c', os.path.join(SRC, f), '-o', '/dev/null'], capture_output=True, text=True)
         if r.returncode != 0:
             sys.exit(r.stderr[-2000:])
