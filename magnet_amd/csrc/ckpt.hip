@@ -378,6 +378,8 @@ struct GramPlan {
     int64_t slab_rows;
 };
 
+constexpr int64_t kMostResults = int64_t(1) << 24;        // m n: what follows counts tiles and their workgroups in 32 bits
+
 // Tile: 64 or 128 rows of a small result, 384 where that saves a second conversion of G, else 256; 32, 64 or 128 columns.
 GramPlan gram_plan(int64_t rows, int32_t m, int32_t n) {
     GramPlan p;
@@ -464,7 +466,7 @@ extern "C" int mh_ckpt_restore(const uint8_t* codes, const uint8_t* scales, int6
 }
 
 extern "C" size_t mh_ckpt_gram_workspace_bytes(int64_t n_rows, int32_t m, int32_t n) {
-    if (n_rows <= 0 || m < 1 || n < 1) return 0;
+    if (n_rows <= 0 || m < 1 || n < 1 || int64_t(m) * n > kMostResults) return 0;
     const GramPlan p = gram_plan(2 * n_rows, m, n);
     return size_t(p.slabs) * p.tiles_m * p.tiles_n * p.bm * p.bn * sizeof(float);
 }
@@ -473,7 +475,7 @@ extern "C" int mh_ckpt_gram(const uint8_t* codes, const uint8_t* scales, int64_t
                             int64_t img, int32_t n, float* out, void* workspace, size_t workspace_bytes, void* stream_) {
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     if (int rc = check_checkpoint(codes, scales, n_rows, m)) return rc;
-    MH_REQUIRE(n >= 1 && int64_t(m) * n <= (int64_t(1) << 24), "m=%d n=%d", m, n);
+    MH_REQUIRE(n >= 1 && int64_t(m) * n <= kMostResults, "m=%d n=%d", m, n);
     MH_REQUIRE(out, "null pointer");
     MH_REQUIRE(ldg >= 0 && img >= 0 && ldg <= (1 << 24) && img <= (int64_t(1) << 40), "row stride of G: %lld", (long long)ldg);
     GramArgs a{};

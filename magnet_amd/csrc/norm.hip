@@ -36,6 +36,7 @@ constexpr int kStats = 5;                  // re mean (high, low), im mean (high
 // 200k x 64 together 183 -> 167 us).  Smaller ones stay, for the convolution that comes next.
 constexpr int64_t kPast = int64_t(64) << 20;
 constexpr int64_t kFewPieces = 64;
+constexpr int32_t kMostGraphs = 1 << 22, kMostChannels = 1 << 20;
 constexpr int kMostParts = 16;             // shares of a graph's pieces
 
 struct NormArgs {
@@ -554,9 +555,9 @@ Workspace workspace_of(int64_t rows, int32_t graphs, int32_t F, int32_t groups) 
 }
 
 int check_norm(int64_t rows, int32_t F, int32_t groups, const void* ptr, int32_t graphs) {
-    MH_REQUIRE(rows >= 0 && rows <= INT32_MAX && F >= 1 && F <= (1 << 20), "n_rows=%lld F=%d", (long long)rows, F);
+    MH_REQUIRE(rows >= 0 && rows <= INT32_MAX && F >= 1 && F <= kMostChannels, "n_rows=%lld F=%d", (long long)rows, F);
     MH_REQUIRE(groups >= 1 && F % groups == 0, "%d channels do not divide into %d groups", F, groups);
-    MH_REQUIRE(graphs >= (rows > 0 ? 1 : 0) && graphs <= (1 << 22) && int64_t(graphs) * groups <= (int64_t(1) << 25), "n_graphs=%d", graphs);
+    MH_REQUIRE(graphs >= (rows > 0 ? 1 : 0) && graphs <= kMostGraphs && int64_t(graphs) * groups <= (int64_t(1) << 25), "n_graphs=%d", graphs);
     MH_REQUIRE(ptr || graphs <= 1, "n_graphs=%d without graph_ptr", graphs);
     return MH_OK;
 }
@@ -602,7 +603,7 @@ void run_pass(Pass pass, const Layout& l, NormArgs a, hipStream_t stream) {
 }  // namespace
 
 extern "C" size_t mh_group_norm_workspace_bytes(int64_t n_rows, int32_t n_graphs, int32_t F, int32_t groups) {
-    if (n_rows < 0 || n_graphs < 0 || F < 1 || groups < 1 || F % groups) return 0;
+    if (n_rows < 0 || n_rows > INT32_MAX || n_graphs < 0 || n_graphs > kMostGraphs || F < 1 || F > kMostChannels || groups < 1 || F % groups) return 0;
     return workspace_of(n_rows, n_graphs, F, groups).bytes;
 }
 

@@ -26,6 +26,7 @@ constexpr int kBlock = 256;
 constexpr int kPer = 8;                    // classes a lane holds at a time
 constexpr int kMore = 24;                  // the same where a row of more than 64 classes fits a few lanes that way
 constexpr int kMostTop = 16;
+constexpr int32_t kMostClasses = 1 << 24;
 constexpr unsigned kMostSums = 2048;       // workgroups that leave a partial sum of the loss: 8 of 4 waves for each CU
 constexpr unsigned kMostBlocks = 1u << 20;
 
@@ -532,7 +533,7 @@ void launch_nll(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
 
 int check_scores(const void* x, int dtype, int64_t n_batch, int64_t n_inner, int32_t classes, int64_t sb, int64_t sc, int64_t sn) {
     MH_REQUIRE(dtype >= 0 && dtype <= 2, "dtype=%d: 0 (float32), 1 (bfloat16) and 2 (float16) are known", dtype);
-    MH_REQUIRE(n_batch >= 0 && n_inner >= 0 && classes >= 1, "n_batch=%lld n_inner=%lld classes=%d", (long long)n_batch, (long long)n_inner, classes);
+    MH_REQUIRE(n_batch >= 0 && n_inner >= 0 && classes >= 1 && classes <= kMostClasses, "n_batch=%lld n_inner=%lld classes=%d", (long long)n_batch, (long long)n_inner, classes);
     MH_REQUIRE(sb >= 0 && sc >= 0 && sn >= 0, "negative stride");
     MH_REQUIRE(n_batch == 0 || n_inner == 0 || x, "scores is null");
     return MH_OK;

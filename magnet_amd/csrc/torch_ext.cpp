@@ -434,6 +434,7 @@ Tensor ckpt_gram(const Tensor& codes, const Tensor& scales, int64_t m, const Ten
     TORCH_CHECK(codes.dim() == 2 && codes.size(0) == 2 * g.n, "G has ", g.n, " rows, the checkpoint ", codes.dim() == 2 ? codes.size(0) / 2 : -1);
     Held h = held(codes, scales, g.n, m);
     TORCH_CHECK(g.f >= 1, "G has no columns");
+    TORCH_CHECK(m * g.f <= (1 << 24), "a product of ", m, " and ", g.f, " columns has more than 2^24 results");
     const size_t bytes = mh_ckpt_gram_workspace_bytes(g.n, int32_t(m), int32_t(g.f));
     Tensor out = at::empty({m, g.f}, G.options());
     Tensor ws = at::empty({int64_t(bytes / sizeof(float))}, G.options());

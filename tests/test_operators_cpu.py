@@ -182,3 +182,17 @@ def test_fused_loss_takes_no_other_criterion():
     for c in (torch.nn.MSELoss(), torch.nn.NLLLoss(reduction='sum'), torch.nn.NLLLoss(weight=torch.ones(3)), torch.nn.NLLLoss(ignore_index=0)):
         with pytest.raises(ValueError):
             _check_fused(True, c)
+
+
+def test_sizes_beyond_the_limits():
+    """Workspace queries and entry points at the ends of their types: 0 and an error, no overflow and no division by its result."""
+    lib = _lib()
+    top = 2 ** 31 - 1
+    for m in (1 << 23, 1 << 24, top):
+        for n in (1 << 23, 1 << 24, top):
+            assert lib.mh_ckpt_gram_workspace_bytes(5, m, n) == 0
+    assert lib.mh_ckpt_gram_workspace_bytes(5, 1 << 12, 1 << 12) > 0
+    _says(lib, lib.mh_ckpt_gram(FAKE, FAKE, 5, 1 << 24, FAKE, 8, 4, 1 << 24, FAKE, FAKE, 1 << 40, None), -1, b'n=')
+    for n, graphs, f in ((2 ** 62, 1, 8), (10, top, 8), (10, 1, top), (10, 1, top - 1)):
+        assert lib.mh_group_norm_workspace_bytes(n, graphs, f, 1) == 0
+    _says(lib, lib.mh_class_logprobs(FAKE, 0, 1, 10, top, 0, 1, 5, None, -100, None, FAKE, None, 0, None, None, 0, 1, 0, None), -1, b'classes')
