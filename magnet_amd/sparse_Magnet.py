@@ -71,7 +71,10 @@ def parse_args(argv=None):
     parser.add_argument('--report', type=int, default=0, metavar='TOP',
                         help='(not in the reference) also write report{split}.npz: log probability of the label, entropy '
                              'and the TOP best classes of every node under the best checkpoint')
-    return parser.parse_args(argv)
+    args = parser.parse_args(argv)
+    if args.report < 0 or args.norm_groups < 0 or (args.norm_groups and args.num_filter % args.norm_groups):
+        parser.error('--report and --norm_groups are not negative, and norm_groups divides num_filter')
+    return args
 
 
 def sparse_mx_to_torch_sparse_tensor(sparse_mx):

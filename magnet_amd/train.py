@@ -130,8 +130,8 @@ class SharedForwardEpochs:
     what node_epoch / link_epoch give (the first epoch makes one extra trunk pass); full-batch models with K orders
     per layer save half of their forward SpMMs.
 
-    The kept pass is used only while the parameters and the input tensors are the objects and versions it was made
-    from (optimizer steps made elsewhere, load_state_dict, in-place writes to X invalidate it); reset() drops it.
+    The kept pass is used only while the parameters, the input tensors and the model's graph_ptr are the objects and versions
+    it was made from (optimizer steps made elsewhere, load_state_dict, in-place writes to X invalidate it); reset() drops it.
     Memory: the saved activations of one forward stay alive between epochs (the peak — one training forward — is
     unchanged).  Not for GraphedEpoch: the first epoch differs from the others.  `fused_loss` as in node_epoch."""
 
@@ -144,6 +144,8 @@ class SharedForwardEpochs:
 
     def _key(self, X_real, X_img):
         ts = [X_real, X_img] + list(self.model.parameters())
+        if getattr(self.model, 'graph_ptr', None) is not None:       # the norms' graphs
+            ts.append(self.model.graph_ptr)
         return tuple((id(t), t._version) for t in ts)
 
     def _trunk(self, X_real, X_img):
@@ -160,7 +162,8 @@ class SharedForwardEpochs:
     def _evaluation_trunk(self, X_real, X_img):
         self.model.eval()
         p = self.model.trunk(X_real, X_img)              # recorded: the next epoch backpropagates through it
-        self._kept = (self._key(X_real, X_img), p, X_real, X_img)     # the inputs held: their ids stay theirs
+        # the inputs held: their ids stay theirs
+        self._kept = (self._key(X_real, X_img), p, X_real, X_img, getattr(self.model, 'graph_ptr', None))
         return p.detach()
 
     def node_epoch(self, X_real, X_img, label, train_index, val_index, criterion=None):

@@ -196,3 +196,47 @@ def test_sizes_beyond_the_limits():
     for n, graphs, f in ((2 ** 62, 1, 8), (10, top, 8), (10, 1, top), (10, 1, top - 1)):
         assert lib.mh_group_norm_workspace_bytes(n, graphs, f, 1) == 0
     _says(lib, lib.mh_class_logprobs(FAKE, 0, 1, 10, top, 0, 1, 5, None, -100, None, FAKE, None, 0, None, None, 0, 1, 0, None), -1, b'classes')
+
+
+def test_drivers_refuse_bad_arguments_at_once():
+    from magnet_amd import Edge_sparseMagnet, sparse_Magnet
+    for driver in (sparse_Magnet, Edge_sparseMagnet):
+        for bad in (['--report', '-1'], ['--norm_groups', '-2'], ['--norm_groups', '3', '--num_filter', '8'], ['--checkpoint_bits', '4']):
+            with pytest.raises(SystemExit):
+                driver.parse_args(bad)
+        assert driver.parse_args(['--report', '2', '--norm_groups', '4', '--num_filter', '8']).report == 2
+
+
+def test_kept_forward_pass_belongs_to_its_graphs():
+    """SharedForwardEpochs: another graph_ptr, or the same one written in place, makes a new pass."""
+    from magnet_amd.train import SharedForwardEpochs
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = torch.nn.Parameter(torch.ones(()))
+            self.register_buffer('graph_ptr', torch.tensor([0, 4, 8]), persistent=False)
+            self.passes = 0
+
+        def trunk(self, real, imag):
+            self.passes += 1
+            return self.w * real * float(self.graph_ptr[1])
+
+        def head(self, p):
+            return torch.log_softmax(p.t().unsqueeze(0), 1)
+    net = Net()
+    epochs = SharedForwardEpochs(net, torch.optim.SGD(net.parameters(), lr=0.1))
+    x, label, index = torch.randn(8, 3), torch.zeros(1, 8, dtype=torch.int64), torch.arange(8)
+    run = lambda: epochs.node_epoch(x, x, label, index, index)
+    run()
+    assert net.passes == 2
+    run()
+    assert net.passes == 3                                         # the evaluation's only
+    net.graph_ptr[1] = 2
+    run()
+    assert net.passes == 5
+    net.graph_ptr = torch.tensor([0, 2, 8])
+    run()
+    assert net.passes == 7
+    run()
+    assert net.passes == 8
