@@ -10,8 +10,8 @@
 // Two passes over the rows per direction: sums, then the elementwise result.  Rows are cut into tiles of T rows and at the
 // graphs' borders; piece d = tile + graph in the merged order of both kinds of border, so a workgroup finds its piece by one
 // binary search in ptr and nothing is planned on the host.  A thread keeps its channels (4, 2 or 1, as the width divides)
-// while it walks down its rows; sums are held in 64 bits (a group may hold 10^8 values, and mean |z|^2 - |m|^2 loses what the
-// mean exceeds the deviation by), joined through LDS and then over the pieces in a fixed order: no atomics, the same result
+// while it walks down its rows; sums are held in 64 bits (a group may hold 10^8 values) and taken of z - z0, z0 the group's
+// first value: mean |z|^2 - |m|^2 loses twice the digits that the mean exceeds the deviation by; they are joined through LDS and then over the pieces in a fixed order: no atomics, the same result
 // every time.  The mean is kept as the sum of two floats, so z - m is exact to 32 bits however far the mean lies from 0.
 // Rows behind the last graph (a padded batch) get zeros, forward and backward.
 //
@@ -223,12 +223,19 @@ __global__ void __launch_bounds__(kBlock) norm_sums_kernel(const NormArgs a) {
     double acc[3][V] = {};
     if (c < a.F) {
         const int step = kBlock / a.lanes;
+        double origin[2][V];
+        const float* first = a.x + row_start(a, p.graph) * a.ld;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int32_t at = (c + j) / a.D * a.D;
+            origin[0][j] = first[at]; origin[1][j] = first[a.im + at];
+        }
 #pragma unroll 4
         for (int64_t row = p.lo + threadIdx.x / a.lanes; row < p.hi; row += step) {
             const Vec<V> re = load<V>(a.x + row * a.ld + c), im = load<V>(a.x + row * a.ld + a.im + c);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const double r = re.v[j], i = im.v[j];
+                const double r = re.v[j] - origin[0][j], i = im.v[j] - origin[1][j];
                 acc[0][j] += r;
                 acc[1][j] += i;
                 acc[2][j] = fma(r, r, fma(i, i, acc[2][j]));
@@ -273,11 +280,15 @@ __device__ inline void join3(double (&v)[3]) {
     }
 }
 
-__device__ inline void leave_stats(const NormArgs& a, int32_t b, int32_t g, int64_t n, const double (&v)[3]) {
+__device__ inline void leave_stats(const NormArgs& a, int32_t b, int32_t g, int64_t lo, int64_t n, const double (&v)[3]) {
     const double count = double(n) * a.D;
-    const double mr = n ? v[0] / count : 0.0, mi = n ? v[1] / count : 0.0;
+    double mr = n ? v[0] / count : 0.0, mi = n ? v[1] / count : 0.0;
     double var = n ? v[2] / count - mr * mr - mi * mi : 0.0;
     if (var < 0.0) var = 0.0;                                       // NaN stays
+    if (n) {
+        const float* first = a.x + lo * a.ld + g * a.D;
+        mr += double(first[0]); mi += double(first[a.im]);
+    }
     float* s = a.stats + (int64_t(b) * a.groups + g) * kStats;
     s[0] = float(mr); s[1] = float(mr - double(float(mr)));
     s[2] = float(mi); s[3] = float(mi - double(float(mi)));
@@ -303,7 +314,7 @@ __global__ void __launch_bounds__(1024) norm_stats_kernel(const NormArgs a) {
         }
     }
     join3(v);
-    if (threadIdx.x == 0) leave_stats(a, b, g, hi - lo, v);
+    if (threadIdx.x == 0) leave_stats(a, b, g, lo, hi - lo, v);
 }
 
 // KEEP (V = 4, F a multiple of 32): also leaves a checkpoint of x, whose values are here anyway.  The 8 threads of a block of 32

@@ -384,7 +384,7 @@ __device__ inline RowGrad row_grad(const GradArgs& a, int64_t row, int64_t b, in
     r.m = st.x;
     r.log_s = st.y;
     if (!any) { r.a = 0.0f; r.log_s = INFINITY; }
-    else if (st.y != st.y) r.a = NAN;
+    else if (!(st.y >= 0.0f)) r.a = NAN;                            // log s of a row with a largest value is at least 0
     return r;
 }
 

@@ -14,14 +14,18 @@
 // `torch.ops.magnet.*` are the calls that replace them.
 #include <cstdint>
 #include <tuple>
+#include <unordered_set>
 #include <utility>
 #include <vector>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/library.h>
 
 #include "../../include/magnet_hip.h"
@@ -536,6 +540,34 @@ variable_list once(variable_list grads, const char* what) {
     return (*error)(std::move(grads));
 }
 
+// A backward pass that is captured into a HIP graph cannot add to leaves on the default stream; their accumulation lies there while
+// an eager pass over the same leaves is alive, and the process would end when the engine came to it.  Asked by the gradients
+// here, which run before the leaves that lie below them; costs a look at the stream where nothing is captured.
+void check_capture() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto* wanted = torch::autograd::get_current_graph_task_exec_info();       // empty: all leaves
+    std::vector<torch::autograd::Node*> todo{torch::autograd::get_current_node().get()};
+    std::unordered_set<torch::autograd::Node*> seen(todo.begin(), todo.end());
+    while (!todo.empty()) {
+        torch::autograd::Node* node = todo.back();
+        todo.pop_back();
+        if (!node) continue;
+        if (dynamic_cast<torch::autograd::AccumulateGrad*>(node)) {
+            bool runs = !wanted || wanted->empty();
+            if (!runs) {
+                const auto it = wanted->find(node);
+                runs = it != wanted->end() && it->second.needed_;
+            }
+            const auto stream = node->stream();
+            TORCH_CHECK(!runs || !stream || stream->id() != 0,                   // 0: the default stream
+                        "a backward pass is being captured while an eager pass over the same leaves is alive: drop that pass's "
+                        "results before the capture");
+        }
+        for (const auto& e : node->next_edges())
+            if (e.function && seen.insert(e.function.get()).second) todo.push_back(e.function.get());
+    }
+}
+
 struct GroupNorm : public torch::autograd::Function<GroupNorm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups,
                           const OptTensor& graph_ptr, double eps, bool relu, int64_t bits, int64_t next_terms) {
@@ -559,6 +591,7 @@ struct GroupNorm : public torch::autograd::Function<GroupNorm> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_capture();
         variable_list s = ctx->get_saved_variables();
         const Tensor &x = s[0], &weight = s[4], &bias = s[5];
         Tensor g = columns(grads[0]);
@@ -684,6 +717,7 @@ struct ClassLogprobs : public torch::autograd::Function<ClassLogprobs> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_capture();
         variable_list v = ctx->get_saved_variables();
         const Tensor &scores = v[0], &labels = v[1], &stat = v[2], &entropy = v[3], &top_index = v[4];
         const Tensor g_lp = grads.size() > 3 ? grads[3] : Tensor();
@@ -736,6 +770,7 @@ struct ClassNll : public torch::autograd::Function<ClassNll> {
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         if (!grads[0].defined()) return variable_list(4);
+        check_capture();
         variable_list v = ctx->get_saved_variables();
         const Tensor& scores = v[0];
         const c10::DeviceGuard guard(scores.device());

@@ -2,6 +2,8 @@
 
 u = 2^-24 is the rounding of a float32 operation (half a step, relative).  Tolerances are worst-case counts of such roundings
 along the formula; the comment at each says which."""
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -324,6 +326,29 @@ def test_group_norm_far_from_zero_and_without_parameters():
     _close(xd.grad, dx, 22 * U * tol_dx + 1e-300, 'dx')
 
 
+def test_group_norm_very_far_from_zero():
+    """A mean 10^6 deviations from 0 (16 steps of float32 to a deviation): the deviations' own accuracy, and behind rows that are NaN."""
+    from magnet_amd.layer.norm import complex_group_norm
+    n, f, groups = 3000, 20, 4
+    x = torch.randn(n, 2, f, generator=_gen(8)) + 1e6
+    one, zero = torch.ones(f, dtype=torch.float64), torch.zeros(f, dtype=torch.float64)
+    g = torch.randn(n, 2, f, generator=_gen(1))
+    g[2500:] = 0
+    sizes = [1000, 1500]
+    out, dx, _, _, tol_out, tol_dx, _, _ = _norm_reference(x, groups, one, zero, sizes, 1e-5, False, g)
+    xd = x.to(DEV)
+    xd[2500:] = float('nan')
+    xd.requires_grad_()
+    y = complex_group_norm(xd, groups, graph_ptr=torch.tensor([0, 1000, 2500], device=DEV))
+    y.backward(g.to(DEV))
+    # as above; the mean is kept to 2^-48 of itself, the reference's own sums of 15000 values to less than 2^-47 (14 levels of
+    # additions); the deviation of both parts together is sqrt(2): 2^-46 * 10^6 covers both
+    far = 2.0 ** -46 * 1e6
+    _close(y.detach(), out, 9 * U * tol_out + far, 'result')
+    _close(xd.grad, dx, 22 * U * tol_dx + 4 * far * float(tol_dx.max()), 'dx')
+    assert not bool(y[2500:].any()) and not bool(xd.grad[2500:].any())
+
+
 def test_group_norm_gradient_against_differences():
     from magnet_amd.layer.norm import complex_group_norm
     x, w, b = _features(37, 12, seed=2), 0.5 + torch.rand(12, generator=_gen(3)), torch.randn(12, generator=_gen(4))
@@ -583,6 +608,21 @@ def test_scores_with_masks_and_values_that_are_not_finite(layout, classes):
         got = _rowwise(class_logprobs(sd3, labd3).logprob, layout)
         assert bool(torch.isnan(got[0])) and bool(torch.isfinite(got[8]))
         assert bool(torch.isnan(class_nll(sd3[:1] if layout == 'row' else sd3[:, :, :1], labd3[:1] if layout == 'row' else labd3[:, :1])[0]))
+
+
+@pytest.mark.parametrize('layout,classes', [('row', 3), ('row', 16), ('row', 80), ('class', 5), ('row', 1100)])
+def test_gradient_of_a_row_without_a_distribution(layout, classes):
+    """A row of -inf alone has a log probability and an entropy of NaN, and so has its gradient; its neighbours keep theirs."""
+    from magnet_amd.layer.scores import class_logprobs, class_nll
+    s = torch.randn(6, classes, generator=_gen(classes))
+    s[2] = -float('inf')
+    lab = torch.tensor([0, 1, 1, 2, 0, 1])
+    sd, labd = _given(s, lab, layout)
+    for loss in (lambda t: class_nll(t, labd)[0], lambda t: class_logprobs(t, labd).logprob.sum(), lambda t: class_logprobs(t).entropy.sum()):
+        t = sd.clone().requires_grad_()
+        loss(t).backward()
+        d = _rowwise(t.grad, layout)
+        assert bool(torch.isnan(d[2]).all()) and bool(torch.isfinite(d[[0, 1, 3, 4, 5]]).all())
 
 
 def test_scores_without_rows_labels_or_gradients():
@@ -1015,3 +1055,55 @@ def test_operators_share_a_gpu_between_streams_and_threads():
     for i in (0, 1):
         for r in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_capture_beside_an_eager_pass_of_the_same_leaves():
+    """The captured backward pass is refused where the leaves' accumulation lies on the default stream, and works once the eager
+    pass is gone."""
+    from magnet_amd.layer.norm import complex_group_norm
+    from magnet_amd.layer.scores import class_logprobs, class_nll
+    n = 300
+    x = _features(n, 8, seed=1).to(DEV).requires_grad_()
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    v = torch.randn(n, 8, generator=_gen(2)).to(DEV).requires_grad_()
+    lab = torch.randint(0, 8, (n,), generator=_gen(3)).to(DEV)
+    leaves = (x, w, v)
+    ones = {k: torch.ones(k, device=DEV) for k in ((n, 2, 8), (n,), ())}
+    outs = (lambda: complex_group_norm(x * 2, 2, w, relu=True), lambda: class_nll(x[:, 0] + v, lab)[0],
+            lambda: class_logprobs(x[:, 1] + v, lab, top=2).entropy)
+    for out in outs:
+        def backward():
+            y = out()
+            y.backward(ones[tuple(y.shape)])
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            backward()                                             # the libraries' workspaces, the leaves' .grad
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        want = [t.grad.clone() for t in leaves if t.grad is not None]
+        alive = out()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match='eager pass'):
+            with torch.cuda.graph(graph):
+                backward()
+        torch.cuda.synchronize()
+        alive.backward(ones[tuple(alive.shape)])                   # the eager pass itself is whole
+        del alive, graph
+        gc.collect()                                               # the error's frames
+        for t in leaves:
+            t.grad = None
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            backward()
+        for _ in range(3):
+            for t in leaves:
+                if t.grad is not None:
+                    t.grad.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.grad for t in leaves if t.grad is not None]
+            assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+        del graph, got, want
+        for t in leaves:
+            t.grad = None
