@@ -295,7 +295,7 @@ int mh_relu_bwd_to(const float* G, int64_t ld, int64_t im, const uint8_t* mask,
  * codes 4-byte, scales 8-byte aligned.
  *   mh_ckpt_store    X -> codes, scales (all of both arrays is written)
  *   mh_ckpt_restore  codes, scales -> X
- *   mh_ckpt_gram     out[m][n] = A^T G, A the restored matrix [R][m], G row-planar float32 with n columns (stride 0 allowed):
+ *   mh_ckpt_gram     out[m][n] = A^T G, A the restored matrix [R][m], G row-planar float32 with n columns (stride 0 allowed, ldg <= 2^24):
  *                    the weight gradient of a convolution whose propagated input is held in 8 bits.  Products and sums are
  *                    float32; the same result every time.  m * n <= 2^24.  A value of G that is not finite makes its column of out NaN.
  *                    workspace: mh_ckpt_gram_workspace_bytes (0 beyond these limits), contents irrelevant before and after.

@@ -53,8 +53,8 @@ def _tail(model, fused_loss, p, *index):
 
 
 def _scored(scores, label, index):
-    """(loss, accuracy) of a node subset from class scores."""
-    return index.scored(scores) if isinstance(index, NodeTargets) else NodeTargets(label, index).scored(scores)
+    """(loss, accuracy) of a node subset from class scores; a node that an index tensor names twice counts twice."""
+    return index.scored(scores) if isinstance(index, NodeTargets) else class_nll(scores[:, :, index], label[:, index])
 
 
 def _node_stats(answer, label, index, criterion, fused_loss):
@@ -86,7 +86,8 @@ def node_epoch(model, opt, X_real, X_img, label, train_index, val_index, criteri
     tensors (required under GraphedEpoch: boolean indexing synchronises), or NodeTargets made from either
     (same loss and accuracy without the per-epoch gather and scatter; `criterion` is then NLL).
     fused_loss: loss, accuracy and their gradient come from the class scores in one pass each way
-    (magnet_amd.layer.scores.class_nll) instead of through log_softmax.
+    (magnet_amd.layer.scores.class_nll) instead of through log_softmax (without a gather if the indices are NodeTargets; rows
+    labelled -100 count for neither).
     Returns (train_loss, train_acc, val_loss, val_acc) as device scalars (no host sync)."""
     _check_fused(fused_loss, criterion)
     criterion = criterion or torch.nn.NLLLoss()
@@ -273,8 +274,6 @@ class GraphedSharedEpochs:
         """The epoch of node_epoch (same arguments; index tensors or NodeTargets, not boolean masks)."""
         _check_fused(fused_loss, criterion)
         criterion = criterion or torch.nn.NLLLoss()
-        if fused_loss:                                # the targets once, outside the capture
-            train_index, val_index = (t if isinstance(t, NodeTargets) else NodeTargets(label, t) for t in (train_index, val_index))
         return cls(model, opt, lambda: model.trunk(X_real, X_img),
                    lambda p: _node_stats(_tail(model, fused_loss, p), label, train_index, criterion, fused_loss),
                    lambda p: _node_stats(_tail(model, fused_loss, p), label, val_index, criterion, fused_loss), warmup)

@@ -833,6 +833,29 @@ def test_fused_loss_epochs_follow_the_plain_ones(dropout):
         assert np.abs(r - runs[0]).max() <= 1e-2 and np.abs((r - runs[0])[0::2]).max() <= 1e-4
 
 
+@pytest.mark.parametrize('kind', ['twice', 'mask', 'one'])
+def test_fused_loss_of_index_tensors_counts_as_the_plain_one(kind):
+    """An index tensor that names nodes more than once, a boolean mask, a single node."""
+    from magnet_amd.layer.sparse_magnet import ChebNet
+    from magnet_amd.train import node_epoch
+    n = 300
+    lap = _graph(n, 1500)
+    x = torch.randn(n, 3, generator=_gen(1)).to(DEV)
+    lab = torch.randint(0, 5, (1, n), generator=_gen(2)).to(DEV)
+    index = {'twice': torch.tensor([3, 7, 3, 3, 250, 7], device=DEV), 'mask': torch.arange(n, device=DEV) % 3 == 0,
+             'one': torch.tensor([11], device=DEV)}[kind]
+    runs = []
+    for fused in (False, True):
+        net = _net(ChebNet, lap, 3, num_filter=8, label_dim=5, layer=2)
+        opt = torch.optim.SGD(net.parameters(), lr=0.0)
+        stats = [float(v) for v in node_epoch(net, opt, x, x, lab, index, index, fused_loss=fused)]
+        runs.append((stats, [p.grad.clone() for p in net.parameters()]))
+    # a loss is a mean of values below 8 with a few roundings each; gradients are products of as many
+    assert np.abs(np.array(runs[0][0]) - np.array(runs[1][0])).max() <= 64 * U
+    for a, b in zip(runs[0][1], runs[1][1]):
+        assert float((a - b).abs().max()) <= 1e3 * U * float(a.abs().max()) + 1e-9
+
+
 def test_training_epoch_as_hip_graphs_follows_the_eager_one():
     """Norms, 8-bit checkpoints and the fused loss under capture: every replay gives what an eager epoch gives, with the
     program's own work in between."""
