@@ -351,7 +351,7 @@ int mh_group_norm_bwd(const float* X, int64_t ld, int64_t im, const uint8_t* cod
  *                      stat: float[2 * rows] for the backward pass, or NULL.
  *   mh_class_logprobs_bwd  d_scores (type of the scores, strides db / dc / dn) from the gradients of logprob, entropy (strides
  *                      0 or 1; NULL: none) and top_logprob (strides tb / tk / tn; NULL: none)
- *   mh_class_nll       loss: mean of -log p over the rows that are not ignored; accuracy: share of them whose best class is the
+ *   mh_class_nll       loss: mean of -log p over the rows that are not ignored (stat: what mh_class_nll_bwd needs, if anything); accuracy: share of them whose best class is the
  *                      label; inv_count: 1 / their number (DEVICE scalars).  workspace: mh_class_nll_workspace_bytes().
  *   mh_class_nll_bwd   d_scores from the gradient of the mean (DEVICE scalar)
  */

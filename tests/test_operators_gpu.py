@@ -547,6 +547,71 @@ def test_class_nll_and_its_gradient(rows, classes, layout, type_):
     assert float(a) == float(loss) and float(b) == float(acc)
 
 
+@pytest.mark.parametrize('type_', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('batch,inner,classes,gap,special', [(1, 65536, 2, 0, False), (1, 65537, 3, 0, True), (1, 70002, 5, 1, True), (3, 30003, 8, 0, True),
+                                                             (250, 263, 7, 2, False), (1, 300003, 4, 3, True), (2, 40001, 6, 0, False),
+                                                             (1, 65535, 5, 0, True)])
+def test_class_nll_of_many_rows(batch, inner, classes, gap, special, type_):
+    """Class-major scores of few classes: rows that do not divide by 4, `gap` values between the classes' rows (so that every class
+    starts at another alignment), ignored rows, rows without a distribution."""
+    from magnet_amd.layer.scores import class_nll
+    g = _gen(inner + classes)
+    wide = (2 * torch.randn(batch, classes, inner + gap, generator=g)).to(TYPES[type_]).to(DEV)
+    lab = torch.randint(-1, classes, (batch, inner), generator=g)
+    lab[lab < 0] = -100
+    s = wide[:, :, :inner]
+    rows = s.permute(0, 2, 1).reshape(-1, classes).double().cpu()
+    flat = lab.reshape(-1)
+    use = flat >= 0
+    if special:                                                    # rows that nothing counts may hold anything
+        odd = torch.nonzero(~use)[:4, 0]
+        for at, v in zip(odd.tolist(), (float('nan'), float('inf'), -float('inf'), 0.0)):
+            s[at // inner, :, at % inner] = v
+        masked = torch.nonzero(use)[:3, 0]
+        for at in masked.tolist():                                 # a class without probability that is not the label
+            c = (int(flat[at]) + 1) % classes
+            s[at // inner, c, at % inner] = -float('inf')
+            rows[at, c] = -float('inf')
+    sd = s.detach().requires_grad_()
+    loss, acc = class_nll(sd, lab.to(DEV))
+    (3.0 * loss).backward()
+    lp = torch.log_softmax(rows, 1)
+    count = int(use.sum())
+    per_row = -lp[use].gather(1, flat[use].unsqueeze(1)).squeeze(1)
+    finite = torch.where(torch.isfinite(rows), rows, torch.zeros_like(rows))
+    spread = float((finite.amax(1) - finite.amin(1)).max()) + 1
+    loss, acc = loss.detach(), acc.detach()
+    # as for the other layouts
+    tol = (classes + 16) * U + 4 * U * (float(per_row.abs().max()) + spread)
+    assert abs(float(loss) - float(per_row.mean())) <= tol + U * float(per_row.mean())
+    first = torch.sort(rows, dim=1, descending=True, stable=True)[1][:, 0]
+    assert float(acc) == float(torch.tensor(int((first[use] == flat[use]).sum()) / count, dtype=torch.float32))
+    d = torch.zeros_like(rows)
+    d[use] = lp[use].exp()
+    d[use] = d[use].scatter_add(1, flat[use].unsqueeze(1), torch.full((count, 1), -1.0, dtype=torch.float64))
+    d *= 3.0 / count
+    rel = (classes + 24) * U + 4 * U * (spread + lp.abs().clamp(max=1e3))
+    bound = 2 * rel * 3.0 / count + torch.finfo(TYPES[type_]).eps / 2 * d.abs() + (2.0 ** -25 if type_ == 'f16' else 1e-38)
+    got = sd.grad.permute(0, 2, 1).reshape(-1, classes).cpu()
+    _close(got, d, bound, 'gradient')
+    assert not bool(got[~use].any())
+    a, b = class_nll(sd.detach(), lab.to(DEV))
+    assert float(a) == float(loss) and float(b) == float(acc)
+    # a counted row without a distribution, a label out of range: NaN where they are, and nowhere else in the gradient
+    at = int(torch.nonzero(use)[5, 0])
+    for kind in ('masked', 'label'):
+        s2, lab2 = s.detach().clone(), lab.clone()
+        if kind == 'masked':
+            s2[at // inner, :, at % inner] = -float('inf')
+        else:
+            lab2[at // inner, at % inner] = classes
+        s2.requires_grad_()
+        bad = class_nll(s2, lab2.to(DEV))[0]
+        bad.backward()
+        got = torch.isnan(s2.grad.permute(0, 2, 1).reshape(-1, classes)).cpu()
+        assert bool(torch.isnan(bad)) and bool(got[at].all()) and int(got.sum()) == classes
+
+
 @pytest.mark.parametrize('layout,classes', [('row', 5), ('class', 5), ('row', 40), ('class', 40), ('row', 1100)])
 def test_scores_with_masks_and_values_that_are_not_finite(layout, classes):
     from magnet_amd.layer.scores import class_logprobs, class_nll
