@@ -448,13 +448,20 @@ __device__ inline RowGrad row_grad(const GradArgs& a, int64_t row, int64_t b, in
 }
 
 template <bool NLL>
-__device__ inline float score_grad(const GradArgs& a, const RowGrad& r, float x, int32_t c, int32_t shift) {   // class c + shift
+__device__ inline float score_grad(const RowGrad& r, float x, int32_t c) {
     const float lp = fmaxf((x - r.m) - r.log_s, kLowest), p = weight(lp);
-    float g = (c == r.label ? r.gy : 0.0f) - p * (NLL ? r.a : fmaf(r.gh, lp, r.a));
-    if (!NLL && a.g_top)
-        for (int t = 0; t < a.top; ++t)
-            if (a.top_idx[r.at + t * a.tk] == c + shift) g += a.g_top[r.at + t * a.tk];
-    return g;
+    return (c == r.label ? r.gy : 0.0f) - p * (NLL ? r.a : fmaf(r.gh, lp, r.a));
+}
+
+// the alternatives' own gradients, to d[j] of class from + j * step
+template <int P>
+__device__ inline void add_top(const GradArgs& a, int64_t at, int32_t from, int32_t step, float (&d)[P]) {
+    for (int t = 0; t < a.top; ++t, at += a.tk) {
+        const int32_t c = int32_t(a.top_idx[at]) - from;
+        const float g = a.g_top[at];
+#pragma unroll
+        for (int j = 0; j < P; ++j) d[j] += c == j * step ? g : 0.0f;
+    }
 }
 
 template <class T, bool NLL>
@@ -478,10 +485,14 @@ __global__ void __launch_bounds__(kBlock) score_grads(const GradArgs a) {
                 const int32_t c = c0 + j * lanes;
                 if (c < a.classes) v[j] = to_f(x[c * a.sc]);
             }
+            float out[kPer];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) out[j] = c0 + j * lanes < a.classes ? score_grad<NLL>(g, v[j], c0 + j * lanes) : 0.0f;
+            if (!NLL && a.g_top) add_top(a, g.at, c0, lanes, out);
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
                 const int32_t c = c0 + j * lanes;
-                if (c < a.classes) d[c * a.dc] = from_f<T>(score_grad<NLL>(a, g, v[j], c, 0));
+                if (c < a.classes) d[c * a.dc] = from_f<T>(out[j]);
             }
         }
     }
@@ -511,13 +522,20 @@ __global__ void __launch_bounds__(kBlock) score_grads_flat(const GradArgs a) {
     g.label -= c0;                                                  // as an element of this piece
     g1.label = g1.label < 0 ? -1 : g1.label + a.classes - c0;
     const int32_t border = a.classes - c0;
-    Pack out;
+    const int64_t at = g.at;
+    float grad[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         if (e == border) g = g1;
-        float d1 = score_grad<NLL>(a, g, to_f(in.v[e]), e, e < border ? c0 : -border);
-        out.v[e] = from_f<T>(d1);
+        grad[e] = score_grad<NLL>(g, to_f(in.v[e]), e);
     }
+    if (!NLL && a.g_top) {
+        add_top(a, at, c0, 1, grad);
+        if (border < E && row + 1 < a.rows) add_top(a, g1.at, -border, 1, grad);
+    }
+    Pack out;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out.v[e] = from_f<T>(grad[e]);
     if (whole) *reinterpret_cast<Pack*>(d) = out;
     else
         for (int e = 0; e < E; ++e)
