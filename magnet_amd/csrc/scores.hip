@@ -151,7 +151,7 @@ __device__ inline uint64_t take_best(uint32_t (&key)[P], const Group& g, int l) 
 
 // Scores of 16 bits whose classes all lie in registers: order and class fit 32 bits, distinct in a row, and nothing needs to be taken
 // out.  Of the keys below the last best, the nearest has the largest difference to it modulo 2^32 (those above it have the
-// smallest): a subtraction and half a maximum of three for each class (60k x 349 bf16, 5 alternatives: 47 -> 37 us).
+// smallest): a subtraction and half a maximum of three for each class, where taking the best out costs five instructions.
 __device__ inline uint32_t short_bits(float x, __hip_bfloat16) { return __float_as_uint(x) >> 16; }
 __device__ inline uint32_t short_bits(float x, __half) { return __half_as_ushort(__float2half(x)); }
 __device__ inline uint32_t short_bits(float, float) { return 0u; }
@@ -694,7 +694,7 @@ struct Shape {
 };
 
 // Lanes of a row.  Row-major: as many as hold the row at kPer classes each, past 64 classes at kMore each but 16 at least (60k x 349
-// with 5 alternatives: 80 us on 64 lanes of 8, 47 us on 16 of 24).  Class-major: one, unless there are too few rows to fill the GPU.
+// with 5 alternatives: 80 us on 64 lanes of 8, 47 us on 16 of 24 while each load was waited for, 30 us now).  Class-major: one, unless there are too few rows to fill the GPU.
 // A workgroup joins on its rows when even whole wavefronts per row are too few for the GPU and every wave gets classes.
 Shape shape_of(int64_t rows, int32_t classes, int64_t sc, int64_t sn, bool can_join, unsigned most) {
     Shape s;
