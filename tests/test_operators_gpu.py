@@ -675,6 +675,40 @@ def test_scores_with_masks_and_values_that_are_not_finite(layout, classes):
         assert bool(torch.isnan(class_nll(sd3[:1] if layout == 'row' else sd3[:, :, :1], labd3[:1] if layout == 'row' else labd3[:, :1])[0]))
 
 
+@pytest.mark.parametrize('type_', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('layout,classes', [('row', 5), ('class', 7), ('row', 64), ('row', 349), ('class', 40), ('row', 1536), ('row', 1600)])
+def test_order_of_the_alternatives(layout, classes, type_):
+    """Ties to the lower class, -0 equal to 0, NaN of either sign before all, masked classes last and in order."""
+    from magnet_amd.layer.scores import class_logprobs, class_nll
+    s = torch.randint(-3, 4, (8, classes), generator=_gen(classes)).to(TYPES[type_])         # ties everywhere
+    s[1] = s[1] * 0.0                                              # zeros of both signs
+    s[2, 1:] = -float('inf')
+    s[3] = -float('inf')
+    nan = torch.tensor([float('nan')]).to(TYPES[type_])
+    s[4, 2], s[4, 4] = nan[0], -nan[0]
+    s[5, classes - 1] = float('inf')
+    tiny = torch.finfo(TYPES[type_]).smallest_normal
+    s[6] = torch.randint(-2, 3, (classes,), generator=_gen(1)).to(TYPES[type_]) * tiny
+    s[7] = torch.randn(classes, generator=_gen(2)).to(TYPES[type_])
+    lab = torch.zeros(8, dtype=torch.int64)
+    top = min(16, classes)
+    sd, labd = _given(s, lab, layout)
+    r = class_logprobs(sd, labd, top=top)
+    inf = float('inf')
+    order = torch.sort(torch.nan_to_num(s.double() + 0.0, nan=inf, posinf=inf, neginf=-inf), dim=1, descending=True, stable=True)[1][:, :top]
+    got = _rowwise(r.top_index, layout)
+    assert torch.equal(got, order)
+    value, lp = _rowwise(r.top_logprob, layout).double(), torch.log_softmax(s.double(), 1).gather(1, order)
+    for i in (0, 1, 2, 6, 7):
+        fine = torch.isfinite(lp[i])
+        assert torch.equal(torch.isfinite(value[i]), fine)
+        assert float((value[i] - lp[i])[fine].abs().max()) <= (classes + 64) * U * 16        # log p below 16, as in the other tests
+    # the best class of the loss is the first of them
+    for i in (0, 1, 6, 7):
+        one = _given(s[i:i + 1], order[i:i + 1, 0], layout)
+        assert float(class_nll(*one)[1]) == 1.0
+
+
 @pytest.mark.parametrize('layout,classes', [('row', 3), ('row', 16), ('row', 80), ('class', 5), ('row', 1100)])
 def test_gradient_of_a_row_without_a_distribution(layout, classes):
     """A row of -inf alone has a log probability and an entropy of NaN, and so has its gradient; its neighbours keep theirs."""
