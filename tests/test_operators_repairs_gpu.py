@@ -1,0 +1,55 @@
+"""Norm, score and checkpoint operators at the places where an earlier form of them went wrong, against 64 bits on the CPU.
+
+u = 2^-24 is the rounding of a float32 operation (half a step, relative).  Tolerances are worst-case counts of such roundings
+along the formula."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = 'cuda'
+U = 2.0 ** -24
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---------------------------------------------------------------------------------------------
+# gradients of single classes far below a row's largest
+# ---------------------------------------------------------------------------------------------
+# unit stride (pieces of 16 bytes), class-major with a lane or more for each row, four rows to a thread, strided, many classes
+@pytest.mark.parametrize('rows,classes,layout', [(300, 5, 'row'), (300, 40, 'row'), (301, 7, 'class'), (70001, 5, 'class'), (65537, 8, 'class'),
+                                                 (130, 12, 'strided'), (9, 1100, 'row'), (40, 100, 'class')])
+def test_small_probabilities_have_their_own_accuracy(rows, classes, layout):
+    """Every element of a gradient is as accurate as its own size asks, however small the class's probability is: scores are halves up
+    to 31.5 on either side, so that x - m is exact."""
+    from magnet_amd.layer.scores import class_logprobs, class_nll
+    s = torch.randint(-63, 64, (rows, classes), generator=_gen(classes)).float() / 2
+    lab = torch.randint(0, classes, (rows,), generator=_gen(rows))
+    lp = torch.log_softmax(s.double(), 1)
+    p, label = lp.exp(), lab.unsqueeze(1)
+    if layout == 'class':
+        given, labels = s.t().contiguous().unsqueeze(0).to(DEV), lab.unsqueeze(0).to(DEV)
+    elif layout == 'strided':
+        wide = torch.zeros(rows, 2 * classes + 1, device=DEV)
+        wide[:, 1::2] = s.to(DEV)
+        given, labels = wide[:, 1::2], lab.to(DEV)
+    else:
+        given, labels = s.to(DEV), lab.to(DEV)
+    back = lambda t: t.detach().cpu()[0].t() if layout == 'class' else t.detach().cpu()
+    # e^t: 2 u of the instruction and 2 u of its correction; a sum of `classes` terms, its additions and its terms' own errors (by
+    # __expf, whose error of |t| 2 u against a share e^-|t| of the sum is below u of it); 2 u of its logarithm, which count as
+    # 2 u log s in e^-log s, 4 u of that; two products and 1 / rows
+    rel = (2 * classes + 20 + 2 * math.log(classes)) * U
+    far = ~torch.zeros(rows, classes, dtype=torch.bool).scatter(1, label, True)
+    t = given.detach().requires_grad_()
+    class_nll(t, labels)[0].backward()
+    got, want = back(t.grad).double(), p / rows
+    assert float(((got - want).abs() / want)[far].max()) <= rel
+    t = given.detach().requires_grad_()
+    class_logprobs(t, labels).logprob.sum().backward()
+    got = back(t.grad).double()
+    assert float(((got + p).abs() / p)[far].max()) <= rel
