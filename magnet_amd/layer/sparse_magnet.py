@@ -305,9 +305,9 @@ class _ChebConvFn(torch.autograd.Function):
             else:                                          # no activation pass: the bias rides on the GEMM
                 torch.addmm(b.reshape(1, cout), _block_rows(block), w.reshape(k1 * cin, cout), out=o2)
                 mask = None
-        ctx.x0 = ctx.held = None
+        ctx.x0 = ctx.held = held = None
         if bits == 8 and not orders_ready and ctx.needs_input_grad[1]:
-            ctx.held = Checkpoint8.store(xp if gemm_first else block)
+            held = Checkpoint8.store(xp if gemm_first else block)
             block = None
         elif (block is not None and not orders_ready and RECOMPUTE_ORDERS_BYTES > 0
                 and 8 * n * k1 * cin > RECOMPUTE_ORDERS_BYTES and ctx.needs_input_grad[1]):
@@ -319,12 +319,16 @@ class _ChebConvFn(torch.autograd.Function):
         ctx.mask = mask
         ctx.block = block
         ctx.shape = (n, cin)
-        ctx.save_for_backward(xp if gemm_first and ctx.held is None else None, weight)
+        # the GEMM-first form leaves what it keeps to autograd, which frees it behind the backward pass (or keeps it, retain_graph);
+        # orders are let go before the backward pass's own recursion
+        if not gemm_first:
+            ctx.held, held = held, None
+        ctx.save_for_backward(xp if gemm_first and held is None else None, weight, held and held.codes, held and held.scales)
         return out
 
     @staticmethod
     def backward(ctx, g):
-        xp, weight = ctx.saved_tensors
+        xp, weight, codes, scales = ctx.saved_tensors
         lap = ctx.lap
         n, cin = ctx.shape
         k1, _, cout = weight.shape
@@ -344,7 +348,7 @@ class _ChebConvFn(torch.autograd.Function):
             if need_w or need_x:
                 _fill_orders(lap, ds)
             if need_w:                                     # X^T [T_0 G ... T_K G] -> [C_in, K+1, C_out]
-                xg = _gram(_rows2(xp), _block_rows(ds)) if ctx.held is None else ctx.held.gram(ds)
+                xg = _gram(_rows2(xp), _block_rows(ds)) if codes is None else Checkpoint8(codes, scales, (n, 2, cin)).gram(ds)
                 dw = xg.view(cin, k1, cout).permute(1, 0, 2).contiguous()
             if need_x:
                 dx = torch.mm(_block_rows(ds), w.transpose(1, 2).reshape(k1 * cout, cin)).view(n, 2, cin)

@@ -53,3 +53,37 @@ def test_small_probabilities_have_their_own_accuracy(rows, classes, layout):
     class_logprobs(t, labels).logprob.sum().backward()
     got = back(t.grad).double()
     assert float(((got + p).abs() / p)[far].max()) <= rel
+
+
+# ---------------------------------------------------------------------------------------------
+# convolutions with 8-bit checkpoints
+# ---------------------------------------------------------------------------------------------
+def _conv(cin, cout, n, k=2, bits=8):
+    from magnet_amd.laplacian import build_magnetic_laplacian, powerlaw_edges
+    from magnet_amd.layer.sparse_magnet import ChebConv
+    from magnet_amd.utils.hermitian import ChebBasis
+    src, dst = powerlaw_edges(n, 3 * n, 3, device=DEV)
+    torch.manual_seed(0)
+    conv = ChebConv(cin, cout, k, ChebBasis(build_magnetic_laplacian(src, dst, n, q=0.15), k), None).to(DEV)
+    conv.checkpoint_bits = bits
+    return conv
+
+
+@pytest.mark.parametrize('cin,cout', [(64, 16), (16, 64)])
+def test_a_backward_pass_lets_its_checkpoint_go(cin, cout):
+    """What a convolution kept is gone behind its backward pass, also while the loss that led there lives on."""
+    n, left = 20000, {}
+    for bits in (32, 8):
+        conv = _conv(cin, cout, n, bits=bits)
+        x = torch.randn(n, 2, cin, generator=_gen(1)).to(DEV)
+        conv.forward_packed(x).sum().backward()                    # plans, library handles, the gradients' memory
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = conv.forward_packed(x, relu=True).sum()
+        kept = torch.cuda.memory_allocated() - before
+        loss.backward()
+        left[bits] = torch.cuda.memory_allocated() - before
+        assert bits == 32 or kept >= 2 * n * cin                   # the codes at least; in 32 bits it may be x itself
+        del loss
+    # the allocator rounds to 512 bytes, a handful of tensors
+    assert left[8] <= left[32] + 4096, left
