@@ -17,6 +17,7 @@ import torch
 from ._lib import ops, MagnetHipError
 
 BLOCK = 32                     # columns that share a scale
+MOST_RESULTS = 1 << 24         # of a `gram`
 
 
 def contiguous_columns(t):
@@ -74,7 +75,8 @@ class Checkpoint8:
         return out.view(self.shape)
 
     def gram(self, g):
-        """A^T G over nodes and parts, A the restored values [2N, m], g row-planar [N, 2, n] float32 -> [m, n]."""
+        """A^T G over nodes and parts, A the restored values [2N, m], g row-planar [N, 2, n] float32 -> [m, n].  At most MOST_RESULTS
+        values of the result, and from one row of g to the next."""
         if g.dim() > 3:
             g = g.flatten(2)
         return ops.ckpt_gram(self.codes, self.scales, self.columns, contiguous_columns(g))

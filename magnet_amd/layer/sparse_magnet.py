@@ -37,7 +37,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .._lib import ops, MagnetHipError
-from ..checkpoint import Checkpoint8
+from ..checkpoint import Checkpoint8, MOST_RESULTS
 from ..laplacian import MagneticLaplacian, build_magnetic_laplacian, pack_complex, _packed_strides
 from ..utils.hermitian import ChebBasis
 
@@ -285,6 +285,10 @@ class _ChebConvFn(torch.autograd.Function):
                                      or in_block.data_ptr() != xp.data_ptr()):
             raise MagnetHipError('in_block must be the contiguous [N, 2, K+1, C_in] block whose order 0 is the input')
         gemm_first = cout < cin and in_block is None
+        keep8 = bits == 8 and not orders_ready and ctx.needs_input_grad[1]
+        if keep8 and max(weight.numel(), 2 * (k1 if gemm_first else 1) * cout) > MOST_RESULTS:       # Checkpoint8.gram's limits
+            raise MagnetHipError('the gradient of a weight [%d, %d, %d] cannot be taken from 8 bits (at most %d values): '
+                                 'checkpoint_bits must be 32' % (k1, cin, cout, MOST_RESULTS))
         out = _alloc_out(n, cout, next_terms, xp.device)
         if gemm_first:
             # one GEMM makes all K+1 matrices X W_k side by side; the SpMM gathers whole rows of an order
@@ -306,7 +310,7 @@ class _ChebConvFn(torch.autograd.Function):
                 torch.addmm(b.reshape(1, cout), _block_rows(block), w.reshape(k1 * cin, cout), out=o2)
                 mask = None
         ctx.x0 = ctx.held = held = None
-        if bits == 8 and not orders_ready and ctx.needs_input_grad[1]:
+        if keep8:
             held = Checkpoint8.store(xp if gemm_first else block)
             block = None
         elif (block is not None and not orders_ready and RECOMPUTE_ORDERS_BYTES > 0

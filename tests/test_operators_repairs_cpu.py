@@ -1,0 +1,21 @@
+"""Refusals and host logic of the norm, score and checkpoint operators that an earlier form of them missed; no GPU."""
+import torch
+
+
+def test_8_bits_are_refused_before_a_forward_whose_gradient_they_cannot_give():
+    """A weight whose gradient has more values than a product with a checkpoint gives: said by the forward pass, not by the
+    backward pass of an epoch.  With 32 bits, or where the weight needs no gradient, the pass goes on (and may stop here for
+    lack of a GPU)."""
+    from magnet_amd import MagnetHipError
+    from magnet_amd.layer.sparse_magnet import _ChebConvFn
+    for k1, cin, cout in ((4, 2048, 2049), (2, 4097, 2048), (1, 1, (1 << 23) + 1)):
+        x, w = torch.zeros(1, 2, cin), torch.zeros(1, 1, 1).expand(k1, cin, cout)
+        for bits, needs in ((8, True), (32, True), (8, False)):
+            said = ''
+            try:
+                _ChebConvFn.apply(x, w.detach().requires_grad_(needs), None, None, False, None, False, 0, bits)
+            except MagnetHipError as e:
+                said = str(e)
+            except Exception:                          # what a host without a GPU and no Laplacian come to
+                pass
+            assert ('checkpoint_bits must be 32' in said) == (bits == 8 and needs), (k1, cin, cout, bits, needs, said)
