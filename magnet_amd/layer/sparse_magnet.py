@@ -814,7 +814,7 @@ class ChebNet(nn.Module):
         """The convolutions and activations: row-planar [N, 2, F] output of the last one.  Nothing in it depends
         on train / eval mode (dropout acts after it), so one trunk pass can serve an evaluation forward and the
         training forward that follows it under the same weights (magnet_amd.train.SharedForwardEpochs)."""
-        return _run_trunk(self.Chebs, real, imag, self.graph_ptr)
+        return _run_trunk(self.Chebs, real, imag, getattr(self, 'graph_ptr', None))      # None: a module pickled without one
 
     def scores(self, p):
         """unwind -> dropout -> Conv1d(2F, label_dim, 1) of a trunk output: class scores [1, label_dim, N], as
@@ -850,7 +850,7 @@ class ChebNet_Edge(nn.Module):
 
     def trunk(self, real, imag):
         """The convolutions and activations (independent of train / eval mode and of the query pairs)."""
-        return _run_trunk(self.Chebs, real, imag, self.graph_ptr)
+        return _run_trunk(self.Chebs, real, imag, getattr(self, 'graph_ptr', None))      # None: a module pickled without one
 
     def scores(self, p, index):
         """pair gather -> dropout -> Linear(4F, label_dim) of a trunk output: class scores [M, label_dim]."""

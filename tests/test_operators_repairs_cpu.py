@@ -1,4 +1,7 @@
 """Refusals and host logic of the norm, score and checkpoint operators that an earlier form of them missed; no GPU."""
+import pickle
+
+import pytest
 import torch
 
 
@@ -19,3 +22,19 @@ def test_8_bits_are_refused_before_a_forward_whose_gradient_they_cannot_give():
             except Exception:                          # what a host without a GPU and no Laplacian come to
                 pass
             assert ('checkpoint_bits must be 32' in said) == (bits == 8 and needs), (k1, cin, cout, bits, needs, said)
+
+
+@pytest.mark.parametrize('name', ['ChebNet', 'ChebNet_Edge'])
+def test_whole_modules_pickled_before_graph_ptr_still_run(name, monkeypatch):
+    """A module object from before the networks had a `graph_ptr` buffer: its trunk is one graph's."""
+    from magnet_amd.layer import sparse_magnet
+    eye = torch.eye(4).to_sparse()
+    net = getattr(sparse_magnet, name)(2, [eye] * 3, [eye] * 3, num_filter=4, K=2, activation=True)
+    state = net.__getstate__() if hasattr(net, '__getstate__') else dict(net.__dict__)
+    state = dict(state, _buffers={k: v for k, v in net._buffers.items() if k != 'graph_ptr'}, _non_persistent_buffers_set=set())
+    old = pickle.loads(pickle.dumps(net))
+    old.__dict__.clear()
+    old.__setstate__(state)
+    monkeypatch.setattr(sparse_magnet, '_run_trunk', lambda *a: a)
+    x = torch.zeros(4, 2)
+    assert old.trunk(x, x)[3] is None and net.trunk(x, x)[3] is None
