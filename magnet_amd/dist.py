@@ -931,6 +931,11 @@ class _OrdersGemmFn(torch.autograd.Function):
         return dz, dw, db, None
 
 
+def _full_precision(convs):
+    if any(getattr(m, 'checkpoint_bits', 32) != 32 for m in convs):
+        raise MagnetHipError('sharded networks keep their activations in 32 bits: checkpoint_bits must be 32')
+
+
 def _sharded_layers(net):
     """(conv, relu follows) of a network that runs sharded."""
     from .layer.norm import ComplexGroupNorm
@@ -938,8 +943,7 @@ def _sharded_layers(net):
     mods, layers, i = list(net.Chebs), [], 0
     if any(isinstance(m, ComplexGroupNorm) for m in mods):
         raise MagnetHipError('sharded networks have no group norm: its statistics would span the ranks')
-    if any(getattr(m, 'checkpoint_bits', 32) != 32 for m in mods):
-        raise MagnetHipError('sharded networks keep their activations in 32 bits: checkpoint_bits must be 32')
+    _full_precision(mods)
     while i < len(mods):
         assert isinstance(mods[i], ChebConv)
         relu = i + 1 < len(mods) and isinstance(mods[i + 1], complex_relu_layer)
@@ -984,6 +988,7 @@ class ShardedChebNet:
 
     def trunk(self, x_rows):
         """x_rows: [rows_me, 2, C_in] row block of the packed input -> [rows_me, 2, F] row block."""
+        _full_precision(c for c, _ in self.layers)           # also where it was set since
         from .layer.sparse_magnet import _ChebTermsFn, _ClenshawFn, _ComplexReluFn
         x, layout = x_rows, 'rows'
         rows_me = self.r1 - self.r0
@@ -1111,6 +1116,7 @@ class RowShardedChebNet(ShardedChebNet):
 
     def trunk(self, x_rows):
         from .layer.sparse_magnet import _ComplexReluFn
+        _full_precision(c for c, _ in self.layers)
         x = x_rows
         rows_me = self.r1 - self.r0
         for i, (conv, relu) in enumerate(self.layers):

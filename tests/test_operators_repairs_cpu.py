@@ -38,3 +38,20 @@ def test_whole_modules_pickled_before_graph_ptr_still_run(name, monkeypatch):
     monkeypatch.setattr(sparse_magnet, '_run_trunk', lambda *a: a)
     x = torch.zeros(4, 2)
     assert old.trunk(x, x)[3] is None and net.trunk(x, x)[3] is None
+
+
+def test_sharded_networks_refuse_8_bits_set_after_they_were_made(monkeypatch):
+    """checkpoint_bits is an attribute of a convolution and may be set at any time: every pass of a sharded network looks."""
+    from magnet_amd import MagnetHipError, dist
+    from magnet_amd.layer.sparse_magnet import ChebNet
+    eye = torch.eye(4).to_sparse()
+    net = ChebNet(2, [eye] * 3, [eye] * 3, num_filter=4, K=2)
+
+    class Part:
+        n, rank, world, group, bounds, r0, r1 = 4, 0, 1, None, (0, 4), 0, 4
+
+    for sharded in (dist.ShardedChebNet(net, None, 4, 0, 1), dist.RowShardedChebNet(net, Part())):
+        net.Chebs[1].checkpoint_bits = 8
+        with pytest.raises(MagnetHipError, match='checkpoint_bits'):
+            sharded.trunk(torch.zeros(4, 2, 2))
+        net.Chebs[1].checkpoint_bits = 32
