@@ -693,6 +693,7 @@ class ChebConv(nn.Module):
                 xp = _PackIntoBlockFn.apply(real, imag, self._n_terms)
                 return self.forward_packed(xp, relu, next_terms, in_block=_block_of(xp, self._n_terms))
             return self.forward_packed(_as_packed(real, imag), relu, next_terms)
+        _kept_bits(self.checkpoint_bits)               # orders that are kept anyway stay in 32, whichever is asked for
         c = getattr(self, '_input_cache', None)
         w = self.weight[:self._n_terms]
         if not (c is not None and c[0] is real and c[1] is imag and c[2] == real._version and c[3] == imag._version
@@ -713,10 +714,9 @@ class ChebConv(nn.Module):
         around `xp`, handed over by the conv before."""
         if self._n_terms > self.weight.size(0):
             raise MagnetHipError('%d Laplacian terms but weight has %d slices' % (self._n_terms, self.weight.size(0)))
-        w = self.weight[:self._n_terms]
+        w, bits = self.weight[:self._n_terms], _kept_bits(self.checkpoint_bits)
         if self._mode == 'cheb':
-            return _ChebConvFn.apply(xp, w, self.bias, self._laps(), relu, in_block, False, next_terms,
-                                     _kept_bits(self.checkpoint_bits))
+            return _ChebConvFn.apply(xp, w, self.bias, self._laps(), relu, in_block, False, next_terms, bits)
         return _ListConvFn.apply(xp.contiguous(), w, self.bias, self._laps(), relu)
 
     def forward(self, data):
@@ -798,7 +798,7 @@ class ChebNet(nn.Module):
     """Node-classification network (reference src/layer/sparse_magnet.py:94-130).  Not in the reference: `norm_groups` > 0 puts
     a ComplexGroupNorm of that many groups behind every convolution, with statistics over each graph of `graph_ptr` (a batch
     of graphs whose Laplacian is block-diagonal; None: one graph); `checkpoint_bits` 8 keeps what the backward pass needs
-    of convolutions and norms in 8 bits (ChebConv.checkpoint_bits)."""
+    of convolutions and norms in 8 bits (ChebConv.checkpoint_bits; convolutions over the reference's lists of matrices keep 32)."""
 
     def __init__(self, in_c, L_norm_real, L_norm_imag, num_filter=2, K=2, label_dim=2, activation=False, layer=2,
                  dropout=False, norm_groups=0, checkpoint_bits=32, graph_ptr=None):

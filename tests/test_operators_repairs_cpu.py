@@ -55,3 +55,20 @@ def test_sharded_networks_refuse_8_bits_set_after_they_were_made(monkeypatch):
         with pytest.raises(MagnetHipError, match='checkpoint_bits'):
             sharded.trunk(torch.zeros(4, 2, 2))
         net.Chebs[1].checkpoint_bits = 32
+
+
+@pytest.mark.parametrize('lists', [True, False])
+def test_bits_other_than_8_and_32_are_refused_by_every_convolution(lists):
+    """Also by one over the reference's lists of matrices, which keeps 32, and by one whose orders the caller keeps."""
+    from magnet_amd import MagnetHipError
+    from magnet_amd.layer.sparse_magnet import ChebConv
+    eye = torch.eye(4).to_sparse()
+    conv = ChebConv(2, 4, 2, [eye] * 3, [eye] * 3)
+    conv.checkpoint_bits = 16
+    if not lists:
+        conv._mode, conv.cache_input_propagation = 'cheb', True
+    for call in (lambda: conv.forward_packed(torch.zeros(4, 2, 2)), lambda: conv.forward_first(torch.zeros(4, 2), torch.zeros(4, 2))):
+        with pytest.raises(MagnetHipError, match='checkpoint_bits' if not lists else 'checkpoint_bits|GPU'):
+            call()
+    with pytest.raises(MagnetHipError, match='checkpoint_bits'):
+        conv.forward_packed(torch.zeros(4, 2, 2))
