@@ -351,8 +351,10 @@ int mh_group_norm_bwd(const float* X, int64_t ld, int64_t im, const uint8_t* cod
  *                      stat: float[2 * rows] for the backward pass, or NULL.
  *   mh_class_logprobs_bwd  d_scores (type of the scores, strides db / dc / dn) from the gradients of logprob, entropy (strides
  *                      0 or 1; NULL: none) and top_logprob (strides tb / tk / tn; NULL: none)
- *   mh_class_nll       loss: mean of -log p over the rows that are not ignored (stat: what mh_class_nll_bwd needs, if anything); accuracy: share of them whose best class is the
- *                      label; inv_count: 1 / their number (DEVICE scalars).  workspace: mh_class_nll_workspace_bytes().
+ *   mh_class_nll       loss: mean of -log p over the rows that are not ignored; accuracy: share of them whose best class is the label;
+ *                      inv_count: 1 / their number (DEVICE scalars).  stat: mh_class_nll_stat_bytes for the backward pass (0: it
+ *                      makes again from the scores what it needs, and stat may be NULL in both), or NULL without one.
+ *                      workspace: mh_class_nll_workspace_bytes().
  *   mh_class_nll_bwd   d_scores from the gradient of the mean (DEVICE scalar)
  */
 int mh_class_logprobs(const void* scores, int dtype, int64_t n_batch, int64_t n_inner, int32_t n_classes, int64_t sb, int64_t sc,
@@ -364,6 +366,7 @@ int mh_class_logprobs_bwd(const void* scores, int dtype, int64_t n_batch, int64_
                           int32_t top, const float* g_top, const int64_t* top_index, int64_t tb, int64_t tk, int64_t tn,
                           void* d_scores, int64_t db, int64_t dc, int64_t dn, void* stream);
 size_t mh_class_nll_workspace_bytes(void);
+size_t mh_class_nll_stat_bytes(int64_t n_batch, int64_t n_inner, int32_t n_classes, int64_t sc, int64_t sn);
 int mh_class_nll(const void* scores, int dtype, int64_t n_batch, int64_t n_inner, int32_t n_classes, int64_t sb, int64_t sc,
                  int64_t sn, const int64_t* labels, int64_t ignore, float* stat, float* loss, float* accuracy,
                  float* inv_count, void* workspace, size_t workspace_bytes, void* stream);

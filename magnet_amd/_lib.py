@@ -112,6 +112,8 @@ def _load():
                                           i64, i64, i64, vp, i64, i64, i64, vp]
     lib.mh_class_nll_workspace_bytes.restype = sz
     lib.mh_class_nll_workspace_bytes.argtypes = []
+    lib.mh_class_nll_stat_bytes.restype = sz
+    lib.mh_class_nll_stat_bytes.argtypes = [i64, i64, i32, i64, i64]
     lib.mh_class_nll.restype = C.c_int
     lib.mh_class_nll.argtypes = [vp, C.c_int, i64, i64, i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, sz, vp]
     lib.mh_class_nll_bwd.restype = C.c_int
@@ -191,7 +193,7 @@ EXPORTS = [
     'mh_pack', 'mh_unpack', 'mh_gather_rows', 'mh_scatter_rows', 'mh_bias_relu', 'mh_relu_bwd', 'mh_relu_bwd_to',
     'mh_ckpt_store', 'mh_ckpt_restore', 'mh_ckpt_gram_workspace_bytes', 'mh_ckpt_gram',
     'mh_group_norm_workspace_bytes', 'mh_group_norm', 'mh_group_norm_bwd',
-    'mh_class_logprobs', 'mh_class_logprobs_bwd', 'mh_class_nll_workspace_bytes', 'mh_class_nll', 'mh_class_nll_bwd',
+    'mh_class_logprobs', 'mh_class_logprobs_bwd', 'mh_class_nll_workspace_bytes', 'mh_class_nll_stat_bytes', 'mh_class_nll', 'mh_class_nll_bwd',
     'mh_exchange_id_bytes', 'mh_exchange_new_id', 'mh_exchange_create', 'mh_exchange_begin', 'mh_exchange_end',
     'mh_exchange_all_gather', 'mh_exchange_destroy',
     'mh_powerlaw_edges', 'mh_stream_read',

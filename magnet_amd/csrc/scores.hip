@@ -834,6 +834,11 @@ extern "C" int mh_class_logprobs_bwd(const void* scores, int dtype, int64_t n_ba
 
 extern "C" size_t mh_class_nll_workspace_bytes(void) { return size_t(kMostSums) * 3 * sizeof(double); }
 
+extern "C" size_t mh_class_nll_stat_bytes(int64_t n_batch, int64_t n_inner, int32_t classes, int64_t sc, int64_t sn) {
+    if (n_batch <= 0 || n_inner <= 0 || in_quads(n_batch * n_inner, n_inner, classes, sc, sn)) return 0;
+    return size_t(n_batch) * size_t(n_inner) * sizeof(float2);
+}
+
 extern "C" int mh_class_nll(const void* scores, int dtype, int64_t n_batch, int64_t n_inner, int32_t classes, int64_t sb, int64_t sc,
                             int64_t sn, const int64_t* labels, int64_t ignore, float* stat, float* loss, float* accuracy,
                             float* inv_count, void* workspace, size_t workspace_bytes, void* stream_) {
@@ -870,7 +875,7 @@ extern "C" int mh_class_nll_bwd(const void* scores, int dtype, int64_t n_batch, 
     if (int rc = check_scores(scores, dtype, n_batch, n_inner, classes, sb, sc, sn)) return rc;
     const int64_t rows = n_batch * n_inner;
     if (rows == 0) return MH_OK;
-    MH_REQUIRE(labels && stat && inv_count && g_loss && d_scores, "null pointer");
+    MH_REQUIRE(labels && (stat || in_quads(rows, n_inner, classes, sc, sn)) && inv_count && g_loss && d_scores, "null pointer");
     MH_REQUIRE(db >= 0 && dc >= 0 && dn >= 0, "negative stride");
     GradArgs a{};
     a.x = scores; a.d = d_scores; a.rows = rows; a.inner = n_inner; a.sb = sb; a.sc = sc; a.sn = sn; a.db = db; a.dc = dc; a.dn = dn;

@@ -755,10 +755,12 @@ struct ClassNll : public torch::autograd::Function<ClassNll> {
         Scores s = scores_of(scores, "scores");
         auto f32 = scores.options().dtype(at::kFloat);
         Tensor loss = at::empty({}, f32), accuracy = at::empty({}, f32), inv_count = at::empty({}, f32), stat;
-        if (keep) stat = at::empty({s.b * s.n, 2}, f32);
+        // nothing where the backward pass makes it again
+        const size_t kept = keep ? mh_class_nll_stat_bytes(s.b, s.n, s.c, s.sc, s.sn) : 0;
+        if (kept) stat = at::empty({int64_t(kept / sizeof(float))}, f32);
         const size_t bytes = mh_class_nll_workspace_bytes();
         Tensor ws = at::empty({int64_t(bytes / sizeof(double))}, f32.dtype(at::kDouble));
-        check_rc(mh_class_nll(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, label_ptr(labels), ignore, keep ? stat.data_ptr<float>() : nullptr,
+        check_rc(mh_class_nll(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, label_ptr(labels), ignore, kept ? stat.data_ptr<float>() : nullptr,
                               loss.data_ptr<float>(), accuracy.data_ptr<float>(), inv_count.data_ptr<float>(), ws.data_ptr(), bytes,
                               stream_of(scores)), "class_nll");
         ctx->set_materialize_grads(false);
@@ -778,7 +780,7 @@ struct ClassNll : public torch::autograd::Function<ClassNll> {
         Tensor d = grad_like(scores);
         Scores ds = scores_of(d, "gradient");
         check_rc(mh_class_nll_bwd(s.p, s.dtype, s.b, s.n, s.c, s.sb, s.sc, s.sn, label_ptr(v[1]), ctx->saved_data["ignore"].toInt(),
-                                  v[2].data_ptr<float>(), v[3].data_ptr<float>(), grads[0].data_ptr<float>(), d.data_ptr(), ds.sb, ds.sc, ds.sn,
+                                  v[2].defined() ? v[2].data_ptr<float>() : nullptr, v[3].data_ptr<float>(), grads[0].data_ptr<float>(), d.data_ptr(), ds.sb, ds.sc, ds.sn,
                                   stream_of(scores)), "class_nll_bwd");
         variable_list out = once({d}, "class_nll");
         out.resize(4);

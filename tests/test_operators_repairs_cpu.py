@@ -72,3 +72,15 @@ def test_bits_other_than_8_and_32_are_refused_by_every_convolution(lists):
             call()
     with pytest.raises(MagnetHipError, match='checkpoint_bits'):
         conv.forward_packed(torch.zeros(4, 2, 2))
+
+
+def test_a_loss_says_what_its_backward_pass_needs():
+    """8 bytes a row, and nothing where the backward pass makes maxima and sums again (few classes, class-major, many rows)."""
+    import ctypes as C
+    from magnet_amd._lib import lib
+    size = lib.mh_class_nll_stat_bytes
+    assert size(1, 2500, 5, 2500, 1) == 8 * 2500 and size(1, 10 ** 6, 3, 1, 3) == 8 * 10 ** 6 and size(1, 10 ** 6, 40, 10 ** 6, 1) == 8 * 10 ** 6
+    assert size(1, 2 * 10 ** 6, 5, 2 * 10 ** 6, 1) == 0 and size(3, 30003, 8, 30003, 1) == 0
+    assert size(0, 5, 5, 5, 1) == 0 and size(1, 0, 5, 5, 1) == 0
+    fake = C.c_void_p(1 << 20)
+    assert lib.mh_class_nll_bwd(fake, 0, 1, 10, 5, 0, 10, 1, fake, -100, None, fake, fake, fake, 0, 10, 1, None) == -1 and b'null' in lib.mh_last_error()

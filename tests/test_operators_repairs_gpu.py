@@ -87,3 +87,31 @@ def test_a_backward_pass_lets_its_checkpoint_go(cin, cout):
         del loss
     # the allocator rounds to 512 bytes, a handful of tensors
     assert left[8] <= left[32] + 4096, left
+
+
+# ---------------------------------------------------------------------------------------------
+# what a loss keeps
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('rows,classes', [(2500, 5), (300000, 5), (300000, 40)])
+def test_a_loss_keeps_what_its_backward_pass_reads(rows, classes):
+    """Nothing for each row where the backward pass makes it again; through raw pointers with no memory for it, the same gradient."""
+    from magnet_amd._lib import lib, ptr, stream_ptr, check
+    from magnet_amd.layer.scores import class_nll
+    s = torch.randn(1, classes, rows, generator=_gen(1)).to(DEV).requires_grad_()
+    lab = torch.randint(0, classes, (1, rows), generator=_gen(2)).to(DEV)
+    class_nll(s, lab)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss, _ = class_nll(s, lab)
+    kept = torch.cuda.memory_allocated() - before
+    size = lib.mh_class_nll_stat_bytes(1, rows, classes, rows, 1)
+    assert (size == 0) == (rows > 10000 and classes == 5) and kept <= size + 4096, (kept, size)
+    loss.backward()
+    if size == 0:
+        out, one, d = torch.empty(3, device=DEV), torch.ones((), device=DEV), torch.empty_like(s)
+        bytes_ = lib.mh_class_nll_workspace_bytes()
+        ws, st = torch.empty(bytes_, dtype=torch.uint8, device=DEV), stream_ptr(torch.device(DEV, 0))
+        args = (ptr(s), 0, 1, rows, classes, 0, rows, 1, ptr(lab), -100, None)
+        check(lib.mh_class_nll(*args, ptr(out), ptr(out[1:]), ptr(out[2:]), ptr(ws), bytes_, st))
+        check(lib.mh_class_nll_bwd(*args, ptr(out[2:]), ptr(one), ptr(d), 0, rows, 1, st))
+        assert float(out[0]) == float(loss.detach()) and torch.equal(d, s.grad)
