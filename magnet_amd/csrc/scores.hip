@@ -648,7 +648,8 @@ __global__ void __launch_bounds__(kBlock) nll_quad_grads(const GradArgs a) {
         for (int r = 0; r < kQuad; ++r) {
             float m, e[C];
             const float inverse = 1.0f / quad_sum<C, true>(v, r, m, e);
-            const bool counted = label[r] != a.ignore;
+            // without a gradient 0 whatever the row holds, as where RowGrad says it
+            const bool counted = label[r] != a.ignore && (scale != 0.0f || label[r] < 0 || label[r] >= C);
             const float gy = label[r] >= 0 && label[r] < C ? scale : NAN;
 #pragma unroll
             for (int c = 0; c < C; ++c) v[c][r] = counted ? (c == label[r] ? gy : 0.0f) - e[c] * inverse * gy : 0.0f;

@@ -115,3 +115,20 @@ def test_a_loss_keeps_what_its_backward_pass_reads(rows, classes):
         check(lib.mh_class_nll(*args, ptr(out), ptr(out[1:]), ptr(out[2:]), ptr(ws), bytes_, st))
         check(lib.mh_class_nll_bwd(*args, ptr(out[2:]), ptr(one), ptr(d), 0, rows, 1, st))
         assert float(out[0]) == float(loss.detach()) and torch.equal(d, s.grad)
+
+
+@pytest.mark.parametrize('rows', [2500, 65536, 70001])
+def test_a_gradient_of_zero_reaches_no_row(rows):
+    """A loss that counts for nothing has gradients of 0, in every kernel: also for a row without a distribution, and NaN for a
+    label out of range."""
+    from magnet_amd.layer.scores import class_nll
+    s = torch.randn(1, 5, rows, generator=_gen(1))
+    s[0, :, 7], s[0, 2, 9], s[0, 1, 11] = -float('inf'), float('nan'), float('inf')
+    lab = torch.randint(0, 5, (1, rows), generator=_gen(2))
+    lab[0, 20] = 5
+    s = s.to(DEV).requires_grad_()
+    class_nll(s, lab.to(DEV))[0].backward(torch.zeros((), device=DEV))
+    wrong = torch.zeros(rows, dtype=torch.bool)
+    wrong[20] = True
+    d = s.grad.cpu()[0]
+    assert bool(torch.isnan(d[:, wrong]).all()) and not bool(d[:, ~wrong].any()) and not bool(torch.isnan(d[:, ~wrong]).any())
