@@ -192,7 +192,7 @@ __device__ inline void gated(const NormArgs& a, const Channels<V>& k, int64_t ro
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             xh[p].v[j] = centred(k, p, j, x[p].v[j]) * k.rstd[j];
-            dy[p].v[j] = open ? dy[p].v[j] : 0.0f;
+            dy[p].v[j] *= open ? 1.0f : 0.0f;                       // as the gate of mh_relu_bwd: what is not finite stays visible
         }
     }
 }

@@ -132,3 +132,30 @@ def test_a_gradient_of_zero_reaches_no_row(rows):
     wrong[20] = True
     d = s.grad.cpu()[0]
     assert bool(torch.isnan(d[:, wrong]).all()) and not bool(d[:, ~wrong].any()) and not bool(torch.isnan(d[:, ~wrong]).any())
+
+
+# ---------------------------------------------------------------------------------------------
+# group norm
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('bits', [8, 32])
+@pytest.mark.parametrize('value', [float('nan'), float('inf')])
+def test_a_gradient_that_is_not_finite_shows_behind_a_closed_gate(bits, value):
+    """The joined gate multiplies, as complex_relu_layer does behind a convolution: the same elements are NaN as in a norm and a
+    layer of their own."""
+    from magnet_amd.layer.norm import complex_group_norm
+    from magnet_amd.layer.sparse_magnet import _ComplexReluFn
+    x = torch.randn(50, 2, 8, generator=_gen(1)).to(DEV)
+    w = torch.ones(8, device=DEV)
+    ptr = torch.tensor([0, 20, 50], dtype=torch.int32, device=DEV)
+    closed = torch.nonzero(complex_group_norm(x, 2, graph_ptr=ptr)[:20, 0] < 0)[0]
+    g = torch.randn(50, 2, 8, generator=_gen(2)).to(DEV)
+    g[closed[0], 1, closed[1]] = value
+    grads = []
+    for joined in (True, False):
+        xr, wr, br = (t.clone().requires_grad_() for t in (x, w, torch.zeros_like(w)))
+        y = complex_group_norm(xr, 2, wr, br, graph_ptr=ptr, relu=joined, checkpoint_bits=bits)
+        (y if joined else _ComplexReluFn.apply(y)).backward(g)
+        grads.append((xr.grad, wr.grad, br.grad))
+    for a, b in zip(*grads):
+        assert torch.equal(torch.isnan(a), torch.isnan(b)) and bool(torch.isnan(b).any())
+        assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
