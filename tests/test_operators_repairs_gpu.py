@@ -159,3 +159,25 @@ def test_a_gradient_that_is_not_finite_shows_behind_a_closed_gate(bits, value):
     for a, b in zip(*grads):
         assert torch.equal(torch.isnan(a), torch.isnan(b)) and bool(torch.isnan(b).any())
         assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
+
+
+@pytest.mark.parametrize('n,f,groups,relu,bits', [(300007, 30, 5, False, 32), (200001, 30, 5, True, 8)])
+def test_group_norm_of_a_large_graph_with_odd_channels(n, f, groups, relu, bits):
+    """Two channels to a thread, sums over a million values, against the definition evaluated on the CPU."""
+    import test_operators_gpu as T
+    from magnet_amd.layer.norm import complex_group_norm
+    x, g = T._features(n, f, seed=n), torch.randn(n, 2, f, generator=_gen(5)) / n
+    w, b = 0.5 + torch.rand(f, generator=_gen(f)), torch.rand(f, generator=_gen(f + 1)) - 0.3
+    x = T._off_the_gate(x, groups, w.double(), b.double(), [n], 1e-5) if relu else x
+    held = torch.from_numpy(T._restored(x)) if bits == 8 else None
+    out, dx, dw, db, tol_out, tol_dx, mag_w, mag_b = T._norm_reference(x, groups, w.double(), b.double(), [n], 1e-5, relu, g, held)
+    xd, wd, bd = (t.to(DEV).requires_grad_() for t in (x, w, b))
+    y = complex_group_norm(xd, groups, wd, bd, relu=relu, checkpoint_bits=bits)
+    y.backward(g.to(DEV))
+    # the same counts of roundings as for the small graphs: sums are held in 64 bits
+    T._close(y.detach(), out, 8 * U * tol_out + 1e-300, 'result')
+    T._close(xd.grad, dx, 20 * U * tol_dx + 1e-300, 'dx')
+    T._close(wd.grad, dw, 8 * U * mag_w + 1e-300, 'dweight')
+    T._close(bd.grad, db, 4 * U * mag_b + 1e-300, 'dbias')
+    # over all values together: each is within a few roundings, so their norm is
+    assert float((y.detach().double().cpu() - out).norm() / out.norm()) < 2 * U
