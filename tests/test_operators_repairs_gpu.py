@@ -181,3 +181,18 @@ def test_group_norm_of_a_large_graph_with_odd_channels(n, f, groups, relu, bits)
     T._close(bd.grad, db, 4 * U * mag_b + 1e-300, 'dbias')
     # over all values together: each is within a few roundings, so their norm is
     assert float((y.detach().double().cpu() - out).norm() / out.norm()) < 2 * U
+
+
+# ---------------------------------------------------------------------------------------------
+# the C ABI without torch
+# ---------------------------------------------------------------------------------------------
+def test_operators_from_a_plain_cpp_caller():
+    """tests/abi/abi_operators.cpp: the checkpoint, norm and score entry points called from plain C++, results against their
+    formulas in double precision on the host, the memory behind every output untouched."""
+    import os
+    import subprocess
+    from conftest import ROOT
+    exe = os.path.join(ROOT, 'tests', 'abi', 'abi_operators')
+    assert os.path.isfile(exe), 'tests/abi/abi_operators is not built (make -C magnet_amd/csrc)'
+    res = subprocess.run([exe], capture_output=True, text=True, timeout=110)
+    assert res.returncode == 0 and res.stdout.strip().endswith('operators ok'), (res.stdout[-300:], res.stderr[-3000:])

@@ -14,7 +14,7 @@ if [ "${1:-build}" = build ]; then
         -c magnet_amd/csrc/$f.hip -o $D/$f.o || exit 1
   done
   /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -Xarch_host -fsanitize=address $D/*.o -o $D/libmagnet_hip_asan.so -ldl || exit 1
-  for t in abi_client abi_sweep; do
+  for t in abi_client abi_sweep abi_operators; do
     /opt/rocm/bin/hipcc -O1 -g -std=c++17 -Xarch_host -fsanitize=address -DABI_SWEEP_SKIP_TEARDOWN tests/abi/$t.cpp -o $D/${t}_asan -L$D -lmagnet_hip_asan -Wl,-rpath,'$ORIGIN' || exit 1
   done
   rm -f $D/*.o
@@ -27,7 +27,8 @@ else
   ( cd $D
     timeout -k 10 100 ./abi_client_asan 300 5000 8 0.25 > /dev/null 2>> ../../$O; echo "abi_client rc=$?" >> ../../$O
     timeout -k 10 100 ./abi_client_asan 300 5000 8 0.25 exchange 2>> ../../$O | tail -1 >> ../../$O; echo "abi_client exchange rc=${PIPESTATUS[0]}" >> ../../$O
-    timeout -k 10 300 ./abi_sweep_asan >> ../../$O 2>&1; echo "abi_sweep rc=$?" >> ../../$O )
+    timeout -k 10 300 ./abi_sweep_asan >> ../../$O 2>&1; echo "abi_sweep rc=$?" >> ../../$O
+    timeout -k 10 300 ./abi_operators_asan >> ../../$O 2>&1; echo "abi_operators rc=$?" >> ../../$O )
   grep -c "ERROR: AddressSanitizer" $O | sed 's/^/AddressSanitizer reports: /' >> $O
-  tail -15 $O
+  tail -60 $O
 fi
