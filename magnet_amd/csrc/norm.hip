@@ -661,7 +661,7 @@ extern "C" int mh_group_norm_bwd(const float* X, int64_t ld, int64_t im, const u
     if (int rc = check_norm(n_rows, F, groups, graph_ptr, n_graphs)) return rc;
     const bool held = codes != nullptr;
     const bool any = n_rows > 0;
-    MH_REQUIRE(!any || ((X || (codes && scales && (!relu || mask))) && G && stats), "null pointer");
+    MH_REQUIRE(!any || ((held ? scales && (!relu || mask) : X != nullptr) && G && stats), "null pointer");
     MH_REQUIRE(workspace, "null pointer");
     MH_REQUIRE(ld >= 0 && im >= 0 && ldg >= 0 && img >= 0 && (!any || !dX || (lddx >= F && imdx >= F)), "stride smaller than F");
     const Workspace w = workspace_of(n_rows, n_graphs, F, groups);

@@ -84,3 +84,20 @@ def test_a_loss_says_what_its_backward_pass_needs():
     assert size(0, 5, 5, 5, 1) == 0 and size(1, 0, 5, 5, 1) == 0
     fake = C.c_void_p(1 << 20)
     assert lib.mh_class_nll_bwd(fake, 0, 1, 10, 5, 0, 10, 1, fake, -100, None, fake, fake, fake, 0, 10, 1, None) == -1 and b'null' in lib.mh_last_error()
+
+
+def test_a_checkpoint_without_its_scales_or_gate_is_refused_also_beside_x():
+    """codes say that the input is the checkpoint: scales, and the gate of a joined ReLU, are read then, whether X is given or not."""
+    import ctypes as C
+    from magnet_amd._lib import lib
+    fake = C.c_void_p(1 << 20)
+
+    def bwd(x, codes, scales, mask, relu):
+        # 4 bytes of workspace: refused for that, and not run, where the pointers are right
+        return lib.mh_group_norm_bwd(x, 16, 8, codes, scales, mask, 10, 8, 2, None, 1, fake, None, None, relu, fake, 16, 8, fake, 16, 8,
+                                     None, None, fake, 4, None)
+    for x in (fake, None):
+        for args in ((fake, None, None, 0), (fake, None, fake, 1), (fake, fake, None, 1)):
+            assert bwd(x, *args) == -1 and b'null' in lib.mh_last_error(), (x, args)
+        assert bwd(x, fake, fake, None, 0) == -4 and bwd(x, fake, fake, fake, 1) == -4
+    assert bwd(fake, None, None, None, 1) == -4 and bwd(None, None, None, None, 0) == -1
