@@ -297,7 +297,7 @@ int mh_relu_bwd_to(const float* G, int64_t ld, int64_t im, const uint8_t* mask,
  *   mh_ckpt_restore  codes, scales -> X
  *   mh_ckpt_gram     out[m][n] = A^T G, A the restored matrix [R][m], G row-planar float32 with n columns (stride 0 allowed, ldg <= 2^24):
  *                    the weight gradient of a convolution whose propagated input is held in 8 bits.  Products and sums are
- *                    float32; the same result every time.  m * n <= 2^24.  A value of G that is not finite makes its column of out NaN.
+ *                    float32; the same result every time.  m * n <= 2^24, n_rows <= 2^40.  A value of G that is not finite makes its column of out NaN.
  *                    workspace: mh_ckpt_gram_workspace_bytes (0 beyond these limits), contents irrelevant before and after.
  */
 int mh_ckpt_store(const float* X, int64_t ld, int64_t im, int64_t n_rows, int32_t m, uint8_t* codes, uint8_t* scales,
@@ -343,7 +343,7 @@ int mh_group_norm_bwd(const float* X, int64_t ld, int64_t im, const uint8_t* cod
  * src/Edge_sparseMagnet.py:176-183), which the reference runs as separate passes over the scores.
  *
  * scores: dtype 0 float32, 1 bfloat16, 2 float16; element (b, c, i) at b sb + c sc + i sn, row (b, i) of n_batch * n_inner rows.
- * At most 2^24 classes.  labels: int64 [n_batch * n_inner] or NULL; a row whose label is `ignore` has log probability 0 and no gradient; any other
+ * At most 2^24 classes and 2^40 rows.  labels: int64 [n_batch * n_inner] or NULL; a row whose label is `ignore` has log probability 0 and no gradient; any other
  * label outside [0, n_classes) gives NaN.  Scores of -inf have probability 0; a row of nothing else, or one with +inf or NaN,
  * gives NaN.  Computed in float32.
  *   mh_class_logprobs  logprob[rows] (with labels), entropy[rows], the `top` (<= 16) best classes of a row at

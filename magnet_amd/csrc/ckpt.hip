@@ -379,6 +379,7 @@ struct GramPlan {
 };
 
 constexpr int64_t kMostResults = int64_t(1) << 24;        // m n: what follows counts tiles and their workgroups in 32 bits
+constexpr int64_t kMostNodes = int64_t(1) << 40;          // more than any memory; products with sizes and strides stay in 64 bits
 
 // Tile: 64 or 128 rows of a small result, 384 where that saves a second conversion of G, else 256; 32, 64 or 128 columns.
 GramPlan gram_plan(int64_t rows, int32_t m, int32_t n) {
@@ -421,7 +422,7 @@ unsigned grid_of(int64_t items) {
 bool vec_ok(const float* x, int64_t ld, int64_t im, int32_t m) { return (m & 3) == 0 && (ld & 3) == 0 && (im & 3) == 0 && mh_aligned16(x); }
 
 int check_checkpoint(const void* codes, const void* scales, int64_t n_rows, int32_t m) {
-    MH_REQUIRE(n_rows >= 0 && m >= 1 && m <= (1 << 24), "n_rows=%lld m=%d", (long long)n_rows, m);
+    MH_REQUIRE(n_rows >= 0 && n_rows <= kMostNodes && m >= 1 && m <= (1 << 24), "n_rows=%lld m=%d", (long long)n_rows, m);
     if (n_rows == 0) return MH_OK;
     MH_REQUIRE(codes && scales, "null pointer");
     MH_REQUIRE((reinterpret_cast<uintptr_t>(codes) & 3) == 0 && (reinterpret_cast<uintptr_t>(scales) & 7) == 0,
@@ -473,7 +474,7 @@ extern "C" int mh_ckpt_restore(const uint8_t* codes, const uint8_t* scales, int6
 }
 
 extern "C" size_t mh_ckpt_gram_workspace_bytes(int64_t n_rows, int32_t m, int32_t n) {
-    if (n_rows <= 0 || m < 1 || n < 1 || int64_t(m) * n > kMostResults) return 0;
+    if (n_rows <= 0 || n_rows > kMostNodes || m < 1 || n < 1 || int64_t(m) * n > kMostResults) return 0;
     const GramPlan p = gram_plan(2 * n_rows, m, n);
     return size_t(p.slabs) * p.tiles_m * p.tiles_n * p.bm * p.bn * sizeof(float);
 }

@@ -28,6 +28,7 @@ constexpr int kPer = 8;                    // classes a lane holds at a time
 constexpr int kMore = 24;                  // the same where a row of more than 64 classes fits a few lanes that way
 constexpr int kMostTop = 16;
 constexpr int32_t kMostClasses = 1 << 24;
+constexpr int64_t kMostRows = int64_t(1) << 40;               // of all batches
 constexpr unsigned kMostSums = 2048;       // workgroups that leave a partial sum of the loss: 8 of 4 waves for each CU
 constexpr unsigned kMostBlocks = 1u << 20;
 
@@ -773,9 +774,13 @@ void launch_nll(const ScoreArgs& a, const Shape& s, hipStream_t stream) {
     else launch_rows<T, 1, true>(a, s, stream);
 }
 
+bool countable(int64_t n_batch, int64_t n_inner) {
+    return n_batch >= 0 && n_inner >= 0 && n_batch <= kMostRows && (n_batch == 0 || n_inner <= kMostRows / n_batch);
+}
+
 int check_scores(const void* x, int dtype, int64_t n_batch, int64_t n_inner, int32_t classes, int64_t sb, int64_t sc, int64_t sn) {
     MH_REQUIRE(dtype >= 0 && dtype <= 2, "dtype=%d: 0 (float32), 1 (bfloat16) and 2 (float16) are known", dtype);
-    MH_REQUIRE(n_batch >= 0 && n_inner >= 0 && classes >= 1 && classes <= kMostClasses, "n_batch=%lld n_inner=%lld classes=%d", (long long)n_batch, (long long)n_inner, classes);
+    MH_REQUIRE(countable(n_batch, n_inner) && classes >= 1 && classes <= kMostClasses, "n_batch=%lld n_inner=%lld classes=%d", (long long)n_batch, (long long)n_inner, classes);
     MH_REQUIRE(sb >= 0 && sc >= 0 && sn >= 0, "negative stride");
     MH_REQUIRE(n_batch == 0 || n_inner == 0 || x, "scores is null");
     return MH_OK;
@@ -836,7 +841,7 @@ extern "C" int mh_class_logprobs_bwd(const void* scores, int dtype, int64_t n_ba
 extern "C" size_t mh_class_nll_workspace_bytes(void) { return size_t(kMostSums) * 3 * sizeof(double); }
 
 extern "C" size_t mh_class_nll_stat_bytes(int64_t n_batch, int64_t n_inner, int32_t classes, int64_t sc, int64_t sn) {
-    if (n_batch <= 0 || n_inner <= 0 || in_quads(n_batch * n_inner, n_inner, classes, sc, sn)) return 0;
+    if (n_batch <= 0 || n_inner <= 0 || !countable(n_batch, n_inner) || in_quads(n_batch * n_inner, n_inner, classes, sc, sn)) return 0;
     return size_t(n_batch) * size_t(n_inner) * sizeof(float2);
 }
 

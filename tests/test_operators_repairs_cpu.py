@@ -101,3 +101,22 @@ def test_a_checkpoint_without_its_scales_or_gate_is_refused_also_beside_x():
             assert bwd(x, *args) == -1 and b'null' in lib.mh_last_error(), (x, args)
         assert bwd(x, fake, fake, None, 0) == -4 and bwd(x, fake, fake, fake, 1) == -4
     assert bwd(fake, None, None, None, 1) == -4 and bwd(None, None, None, None, 0) == -1
+
+
+def test_row_counts_whose_products_leave_64_bits_are_refused():
+    """Counts are multiplied by each other and by sizes: beyond 2^40 rows every entry point says so, and a workspace query is 0."""
+    import ctypes as C
+    from magnet_amd._lib import lib
+    fake, top = C.c_void_p(1 << 20), 2 ** 63 - 1
+    for n in (2 ** 40 + 1, 2 ** 62, top):
+        assert lib.mh_ckpt_store(fake, 8, 4, n, 4, fake, fake, None) == -1 and b'n_rows' in lib.mh_last_error()
+        assert lib.mh_ckpt_restore(fake, fake, n, 4, fake, 8, 4, None) == -1 and b'n_rows' in lib.mh_last_error()
+        assert lib.mh_ckpt_gram(fake, fake, n, 4, fake, 8, 4, 4, fake, fake, top, None) == -1 and b'n_rows' in lib.mh_last_error()
+        assert lib.mh_ckpt_gram_workspace_bytes(n, 4, 4) == 0
+    assert 0 < lib.mh_ckpt_gram_workspace_bytes(2 ** 40, 384, 128) < 1 << 30
+    for b, n in ((2 ** 32, 2 ** 32), (top, 2), (2, top), (2 ** 21, 2 ** 20), (1, 2 ** 40 + 1)):
+        assert lib.mh_class_logprobs(fake, 0, b, n, 5, 0, 1, 5, None, -100, None, fake, None, 0, None, None, 0, 1, 0, None) == -1
+        assert b'n_inner' in lib.mh_last_error()
+        assert lib.mh_class_nll(fake, 0, b, n, 5, 0, 1, 5, fake, -100, None, fake, fake, fake, fake, 1 << 30, None) == -1
+        assert lib.mh_class_nll_bwd(fake, 0, b, n, 5, 0, 1, 5, fake, -100, fake, fake, fake, fake, 0, 1, 5, None) == -1
+        assert lib.mh_class_nll_stat_bytes(b, n, 5, 1, 5) == 0
