@@ -56,7 +56,7 @@ __device__ inline uint64_t candidate(float x, uint32_t c) { return (uint64_t(ord
 __device__ inline float weight(float x) { return __expf(x); }
 // e^x to 2 units in the last place however far x lies below 0, for a probability that is an answer by itself (a gradient's element):
 // h = fl(x log2 e) is short of x log2 e by r, at most 2^-17, which two fused products give back: e^x = 2^h 2^r = 2^h (1 + r ln 2).
-// Three instructions more (60k x 349 bf16, report and gradient: 55.5 -> 59.6 us; loss of 2M x 5: 36.7 -> 37.3).
+// Three instructions more (gradient of 60k x 349 bf16: 26.4 -> 30.7 us, of the loss of 2M x 5: 16.1 -> 16.4).
 __device__ inline float accurate_weight(float x) {
     constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596303e-8f, kLn2 = 0.693147181f;
     const float h = x * kLog2e, r = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -h)), e = __builtin_amdgcn_exp2f(h);
@@ -419,9 +419,9 @@ struct GradArgs {
 };
 
 // d x_c = [c = y] g_y + sum_t [c = i_t] g_t - p_c (a + g_H log p_c) with a = g_y + sum_t g_t + g_H H: what it takes of a row.
-// p = e^(x-m) / s and not e^(log p): rounding log p to 32 bits would cost p |log p| 2^-24 of itself.  x - m and log p are
-// kept above kLowest, where p is 0 already, so that a class without probability multiplies no infinity; a row without a
-// distribution has a = NaN, one that no gradient reaches has p = 0 whatever it holds.
+// p = e^(x-m) / s and not e^(log p): rounding log p to 32 bits would cost p |log p| 2^-24 of itself.  x - m is kept above
+// kLowest, where p is 0 already, so that a class without probability multiplies no infinity; a row without a distribution has
+// a = NaN, one that no gradient reaches has p = 0 whatever it holds.
 struct RowGrad {
     int64_t at;                             // of the alternatives
     int32_t label;                          // -1: none
@@ -453,15 +453,15 @@ __device__ inline RowGrad row_grad(const GradArgs& a, int64_t row, int64_t b, in
     r.m = st.x;
     r.log_s = st.y;
     r.inverse = accurate_weight(-st.y);
-    if (!any) { r.a = r.inverse = 0.0f; r.log_s = INFINITY; }
+    if (!any) r.a = r.inverse = r.log_s = 0.0f;
     else if (!(st.y >= 0.0f)) r.a = NAN;                            // log s of a row with a largest value is at least 0
     return r;
 }
 
 template <bool NLL>
 __device__ inline float score_grad(const RowGrad& r, float x, int32_t c) {
-    const float t = x - r.m, lp = fmaxf(t - r.log_s, kLowest), p = accurate_weight(fmaxf(t, kLowest)) * r.inverse;
-    return (c == r.label ? r.gy : 0.0f) - p * (NLL ? r.a : fmaf(r.gh, lp, r.a));
+    const float t = fmaxf(x - r.m, kLowest), p = accurate_weight(t) * r.inverse;
+    return (c == r.label ? r.gy : 0.0f) - p * (NLL ? r.a : fmaf(r.gh, t - r.log_s, r.a));
 }
 
 // the alternatives' own gradients, to d[j] of class from + j * step
@@ -710,7 +710,11 @@ struct Shape {
 };
 
 // Lanes of a row.  Row-major: as many as hold the row at kPer classes each, past 64 classes at kMore each but 16 at least (60k x 349
-// with 5 alternatives: 80 us on 64 lanes of 8, 47 us on 16 of 24 while each load was waited for, 30 us now).  Class-major: one, unless there are too few rows to fill the GPU.
+// with 5 alternatives: 80 us on 64 lanes of 8, 47 us on 16 of 24 while each load was waited for, 30 us now).  Class-major: one, unless
+// there are too few rows to fill the GPU.  Measured at 349 classes and kept for its neighbours: a row of 65 classes takes the same 384
+// places.  60k rows in bf16, report with 5 alternatives (loss forward): 65 classes 30 us (25), 128 30 (24), 172 31 (24), 349 32 (25), 500 108
+// (52) and 1000 150 (71), which take strides that are not known when compiled and two waves a SIMD.  Class-major past kPer classes a lane
+// keeps a list of its best classes: 2M x 40 float32 169 us (86), where the read alone takes 68.
 // A workgroup joins on its rows when even whole wavefronts per row are too few for the GPU and every wave gets classes.
 Shape shape_of(int64_t rows, int32_t classes, int64_t sc, int64_t sn, bool can_join, unsigned most) {
     Shape s;
