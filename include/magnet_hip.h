@@ -292,6 +292,8 @@ int mh_relu_bwd_to(const float* G, int64_t ld, int64_t im, const uint8_t* mask,
  *     scales uint8 [mp / 32][Rp], Rp = R rounded up to 8: exponent plus 128 (0 in the rows behind R); 0 marks a block that
  *            held a value that was not finite: its codes are 128 and it is restored as NaN
  * A value is code * 2^exponent, off by at most half a step of its block: at most 1 / 127.5 of the block's largest magnitude.
+ * Exponents lie between -110 and 121: a block below 2^-103 keeps multiples of 2^-110, and a magnitude from 127.5 * 2^121 on may be
+ * off by a whole step.
  * codes 4-byte, scales 8-byte aligned.
  *   mh_ckpt_store    X -> codes, scales (all of both arrays is written)
  *   mh_ckpt_restore  codes, scales -> X

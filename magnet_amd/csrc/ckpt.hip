@@ -6,8 +6,9 @@
 //     codes  uint8 [R][mp], mp = m rounded up to 32 (the columns behind m hold 128)
 //     scales uint8 [mp / 32][Rp], s + 128, Rp = R rounded up to 8 (the rows behind R hold 0); 0: a value of the block was not
 //            finite, and the whole block (of codes 128) is restored as NaN
-// The error of a value is at most 2^s / 2: between 1 / 255 and 1 / 127.5 of its block's largest magnitude.  A power of
-// two costs up to one bit against a free scale and buys that code * 2^s is exact in bf16 (7 bits): the weight gradient runs on
+// The error of a value is at most 2^s / 2: between 1 / 255 and 1 / 127.5 of its block's largest magnitude.  At the ends of s: a block
+// below 2^-103 keeps multiples of 2^-110, and a magnitude from 127.5 2^121 on is held at 127 2^121, up to a whole 2^s away (64 2^122
+// would leave float32).  A power of two costs up to one bit against a free scale and buys that code * 2^s is exact in bf16 (7 bits): the weight gradient runs on
 // the bf16 matrix cores without a further rounding of the activations.  The scales of 8 consecutive rows are 8 consecutive
 // bytes: one load for a thread that holds 8 rows of a block.
 #include <cstdint>
@@ -381,7 +382,9 @@ struct GramPlan {
 constexpr int64_t kMostResults = int64_t(1) << 24;        // m n: what follows counts tiles and their workgroups in 32 bits
 constexpr int64_t kMostNodes = int64_t(1) << 40;          // more than any memory; products with sizes and strides stay in 64 bits
 
-// Tile: 64 or 128 rows of a small result, 384 where that saves a second conversion of G, else 256; 32, 64 or 128 columns.
+// Tile: 64 or 128 rows of a small result, 256 up to 256 columns, beyond 768 and for narrow results, else 384; 32, 64 or 128 columns.
+// 384 rows take 257 to 384 columns with one conversion of G (1M x 384 x 128: 597 us).  Past 384 columns they need two, as 256 rows do up
+// to 512 and with a third of the tiles or more empty: 1M x 512 x 128 takes 1380 us, in tiles of 256 766 us; 768 columns 1410 to 1470 and 1395 us.
 GramPlan gram_plan(int64_t rows, int32_t m, int32_t n) {
     GramPlan p;
     const int32_t mp = (m + 31) & ~31;
@@ -395,7 +398,8 @@ GramPlan gram_plan(int64_t rows, int32_t m, int32_t n) {
     int64_t each = want > 1 ? (rows + want - 1) / want : rows;
     // A sum in the matrix unit's 32 bits runs over 1024 rows of a small tile and bm bn / 4 of a larger one (16 bytes of partial sums
     // to a row), as long as all of them take 64 MB at most: 1.4M nodes x 3 x 46 are off by
-    // 9e-7 of the result in 201 us, in slabs of 2816 rows by 1.5e-6 in 182 us
+    // 9e-7 of the result in 201 us, in slabs of 2816 rows by 1.5e-6 in 182 us.  384 x 128 tiles sum 12288 rows: 1M nodes are off by
+    // 1.6e-6, a float32 product over slabs of 16384 rows by 1.5e-6.
     const int64_t results = int64_t(p.tiles_m) * p.tiles_n * p.bm * p.bn, most = (int64_t(1) << 24) / results;
     const int64_t fits = most > 1 ? (rows + most - 1) / most : rows, tile = p.bm * p.bn / 4 > 1024 ? p.bm * p.bn / 4 : 1024;
     const int64_t longest = fits > tile ? fits : tile;

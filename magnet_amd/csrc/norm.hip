@@ -18,6 +18,11 @@
 // Bound by HBM: the passes read 8 NF and 8 NF bytes and write 8 NF forward, 16 NF + 16 NF and 8 NF backward.  The pass for
 // sums has as many tiles as the GPU holds workgroups at once, the elementwise pass small ones.  The elementwise pass walks the
 // pieces backwards: the rows read last are still in the 256 MB cache in front of the memory.
+//
+// Made for batches of up to a few thousand graphs.  1M x 64 in 8 groups, forward and backward: one graph 264 and 438 us, 512 graphs 284 and
+// 455, 2000 301 and 479, 10000 353 and 612, 50000 766 and 1431, 200000 (5 rows each) 2386 and 5487 us: each graph has pieces of its own to
+// join, and 16 threads to a channel add the graphs' sums for dgamma and dbeta.  The workspace, one size for both
+// directions, is 8 MB at 2000 graphs, 160 MB at 50000 and 635 MB at 200000 beside an input of 512 MB.
 #include <cstdint>
 
 #include <hip/hip_runtime.h>
