@@ -196,3 +196,83 @@ def test_operators_from_a_plain_cpp_caller():
     assert os.path.isfile(exe), 'tests/abi/abi_operators is not built (make -C magnet_amd/csrc)'
     res = subprocess.run([exe], capture_output=True, text=True, timeout=110)
     assert res.returncode == 0 and res.stdout.strip().endswith('operators ok'), (res.stdout[-300:], res.stderr[-3000:])
+
+
+# ---------------------------------------------------------------------------------------------
+# offsets that pass 32 bits
+# ---------------------------------------------------------------------------------------------
+def _wide_gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def test_checkpoints_of_more_than_2_to_32_values():
+    """4.6G values: both ends byte for byte as on their own; the weight gradient as the sum of its halves (all terms positive, so
+    that a bound of 12288 float32 additions is one of the result)."""
+    from magnet_amd.checkpoint import Checkpoint8
+    n, m, k, ends = 6_000_000, 384, 8, 1001
+    x = torch.rand(n, 2, m, device=DEV, generator=_wide_gen(1))
+    g = torch.rand(n, 2, k, device=DEV, generator=_wide_gen(2))
+    ck = Checkpoint8.store(x)
+    assert ck.codes.numel() > 2 ** 32
+    for part, rows in ((slice(0, ends), slice(0, 2 * ends)), (slice(n - ends, n), slice(2 * (n - ends), 2 * n))):
+        own = Checkpoint8.store(x[part])
+        assert torch.equal(own.codes, ck.codes[rows]) and torch.equal(own.scales[:, :2 * ends], ck.scales[:, rows])
+    back = ck.restore()
+    for part in (slice(0, ends), slice(n - ends, n)):
+        assert torch.equal(back[part], Checkpoint8.store(x[part]).restore())
+    del back
+    halves = sum(Checkpoint8.store(x[part]).gram(g[part]).double() for part in (slice(0, n // 2), slice(n // 2, n)))
+    got = ck.gram(g).double()
+    assert float(((got - halves).abs() / halves).max()) <= 2 * (12288 + 8) * U
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_group_norm_of_more_than_2_to_31_values(bits):
+    """The last graph of 2.3G values, forward and backward, as on its own."""
+    from magnet_amd.layer.norm import complex_group_norm
+    n, f, last = 9_000_000, 128, 10007
+    x = torch.randn(n, 2, f, device=DEV, generator=_wide_gen(1)).requires_grad_()
+    g = torch.randn(n, 2, f, device=DEV, generator=_wide_gen(2))
+    ptr = torch.tensor([0, n - last, n], dtype=torch.int32, device=DEV)
+    y = complex_group_norm(x, 8, graph_ptr=ptr, relu=True, checkpoint_bits=bits)
+    y.backward(g)
+    own = x[n - last:].detach().requires_grad_()
+    z = complex_group_norm(own, 8, relu=True, checkpoint_bits=bits)
+    z.backward(g[n - last:])
+    y, z = y.detach(), z.detach()
+    # the same formula on the same values, its 64-bit sums in another order: a rounding of mean and deviation either way; a gate
+    # that opens with it is 0 on one side
+    same = (y[n - last:, :1] == 0) == (z[:, :1] == 0)
+    assert float((~same).sum()) <= 8
+    assert float(((y[n - last:] - z).abs() * same).max()) <= 16 * U * float(z.abs().max())
+    assert float(((x.grad[n - last:] - own.grad).abs() * same).max()) <= 64 * U * float(own.grad.abs().max())
+    assert bool(torch.isfinite(y[::4999]).all()) and bool(torch.isfinite(x.grad[::4999]).all())
+
+
+@pytest.mark.parametrize('rows,classes,layout,dtype', [(60_000_000, 40, 'class', torch.float32), (7_000_000, 349, 'row', torch.bfloat16),
+                                                       (300_000_000, 8, 'class', torch.bfloat16)])
+def test_scores_of_more_than_2_to_31_values(rows, classes, layout, dtype):
+    """The last rows as on their own; the loss as the mean of its halves."""
+    from magnet_amd.layer.scores import class_logprobs, class_nll
+    end, by_class = 1003, layout == 'class'
+    s = torch.empty((1, classes, rows) if by_class else (rows, classes), device=DEV, dtype=dtype).normal_(generator=_wide_gen(1)).requires_grad_()
+    lab = torch.randint(0, classes, (1, rows) if by_class else (rows,), device=DEV, generator=_wide_gen(2))
+    assert s.numel() > 2 ** 31
+    tail = lambda t: t[..., rows - end:] if by_class else t[rows - end:]
+    own = tail(s).detach().contiguous().requires_grad_()
+    loss, acc = class_nll(s, lab)
+    loss.backward()
+    part, _ = class_nll(own, tail(lab).contiguous())
+    (part * (end / rows)).backward()
+    depth = (classes + 32) * U + torch.finfo(dtype).eps              # two values a rounding apart may be two steps of the type apart
+    assert float((tail(s.grad).double() - own.grad.double()).abs().max()) <= depth / rows
+    loss = loss.detach()
+    halves = [class_nll(t.detach(), u) for t, u in ((s[..., :rows // 2], lab[..., :rows // 2]), (s[..., rows // 2:], lab[..., rows // 2:]))] \
+        if by_class else [class_nll(t.detach(), u) for t, u in zip(s.split(rows // 2), lab.split(rows // 2))]
+    assert abs(float(loss) - float(halves[0][0] + halves[1][0]) / 2) <= 8 * U * float(loss)
+    assert abs(float(acc) - float(halves[0][1] + halves[1][1]) / 2) <= 8 * U
+    s.grad = None
+    r, q = class_logprobs(s.detach(), lab, top=2), class_logprobs(own.detach(), tail(lab).contiguous(), top=2)
+    for a, b in ((tail(r.logprob), q.logprob), (tail(r.entropy), q.entropy)):
+        assert float((a - b).abs().max()) <= depth * 16
+    assert torch.equal(r.top_index[..., rows - end:] if by_class else r.top_index[rows - end:], q.top_index)
