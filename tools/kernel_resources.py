@@ -28,7 +28,7 @@ def demangle(names):
 def main():
     print('kernel resource usage, gfx950, hipcc %s' % ' '.join(FLAGS[:4]))
     print('occupancy = waves per SIMD the register and LDS budget allows (8 is the hardware maximum; a CU has 4 SIMDs, 160 KiB of LDS)')
-    print('%-14s %-58s %6s %6s %6s %8s %9s %10s' % ('file', 'kernel', 'VGPRs', 'AGPRs', 'SGPRs', 'scratch', 'LDS bytes', 'waves/SIMD'))
+    print('%-14s %-66s %6s %6s %6s %8s %9s %10s' % ('file', 'kernel', 'VGPRs', 'AGPRs', 'SGPRs', 'scratch', 'LDS KiB', 'waves/SIMD'))
     for f in ['cspmm.hip', 'radix_sort.hip', 'lap_build.hip', 'halo.hip', 'aux.hip', 'ckpt.hip', 'norm.hip', 'scores.hip']:
         r = subprocess.run(['/opt/rocm/bin/hipcc'] + FLAGS + ['-c', os.path.join(SRC, f), '-o', '/dev/null'], capture_output=True, text=True)
         if r.returncode != 0:
@@ -47,8 +47,8 @@ def main():
                 cur[k.strip()] = v.strip()
         names = demangle([r_['name'] for r_ in recs])
         for n, r_ in zip(names, recs):
-            print('%-14s %-58s %6s %6s %6s %8s %9s %10s' % (f, n[:58], r_.get('VGPRs'), r_.get('AGPRs'), r_.get('TotalSGPRs'),
-                                                           r_.get('ScratchSize [bytes/lane]'), r_.get('LDS Size [bytes/block]'),
+            print('%-14s %-66s %6s %6s %6s %8s %9s %10s' % (f, n[:66], r_.get('VGPRs'), r_.get('AGPRs'), r_.get('TotalSGPRs'),
+                                                           r_.get('ScratchSize [bytes/lane]'), '%.2f' % (int(r_.get('LDS Size [bytes/block]', 0)) / 1024),
                                                            r_.get('Occupancy [waves/SIMD]')))
 
 
